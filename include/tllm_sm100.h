@@ -429,6 +429,105 @@ TLLM_API int tllm_qkv_norm_rope(const void *x, const void *w, const void *wq, co
                                 int64_t lda, int64_t ldw, int64_t ldo, float eps, int dtype,
                                 void *stream);
 
+/*
+ * Bookkeeping of one serving step over a paged cache, on the GPU (no counterpart in the reference,
+ * whose callers fill block tables on the host: python/triton_llm/ops/paged_attention.py:92-128).
+ * Sequence b has max(0, seq_lens[b]) tokens in the cache, in the blocks that block_tables[b] names,
+ * and n_new[b] new ones. It takes the blocks it lacks from the front of free_blocks [n_free], in
+ * the order of the sequences, and they are written into block_tables [B, max_blocks] (strides
+ * sbt, elements). For packed token i = cu_seqlens[b] + t (rows up to max_tokens): positions[i] =
+ * seq_lens[b] + t and slots[i] = block * block_size + offset. cu_seqlens [B + 1], new_lens [B],
+ * taken [1]: how many free blocks went. A sequence that max_blocks, n_free or max_tokens cannot
+ * hold is refused whole (slots -1, new_lens the old length, its table row untouched); rows past
+ * the last new token get slot -1 and position 0. At most 16384 sequences; block_size >= 1.
+ */
+TLLM_API int tllm_paged_plan(int32_t *block_tables, const int32_t *seq_lens, const int32_t *n_new,
+                             const int32_t *free_blocks, int32_t *slots, int32_t *positions,
+                             int32_t *cu_seqlens, int32_t *new_lens, int32_t *taken, int64_t B,
+                             int64_t max_blocks, int64_t n_free, int64_t max_tokens,
+                             int64_t block_size, const int64_t *sbt, void *stream);
+
+/*
+ * RMS norm of every head of q [T, Hq, D] and k [T, Hkv, D] (weights wq, wk [D]) and the rotate-half
+ * rotation by positions of 1 to 4 axes, in one pass; a form of rmsnorm_rope
+ * (python/triton_llm/ops/rmsnorm_rope.py:51-75) for packed projections, without its rounding of
+ * the normed value before the rotation. Rotary pair i (elements i and i + D / 2) of token t turns
+ * by cos/sin[positions[a * spos + t], i], a being the pair's axis: bits 2 (i % 16) of the host
+ * array axis_of_pair[i / 16]. cos/sin are fp32 [rope_rows, D / 2], 16-byte aligned rows with
+ * strides scos/ssin. Strides sq/sk/sqo/sko are {token, head}, multiples of 8; innermost 1;
+ * pointers 16-byte aligned; D in {16,32,64,128}. A position outside the table uses row 0 and is
+ * reported through tllm_debug_status.
+ */
+TLLM_API int tllm_qk_norm_rope(const void *q, const void *k, const void *wq, const void *wk,
+                               const float *cos, const float *sin, const int32_t *positions,
+                               void *q_out, void *k_out, int64_t T, int64_t Hq, int64_t Hkv,
+                               int64_t D, int64_t rope_rows, int64_t scos, int64_t ssin,
+                               int64_t axes, int64_t spos, const uint32_t *axis_of_pair,
+                               const int64_t *sq, const int64_t *sk, const int64_t *sqo,
+                               const int64_t *sko, float eps, int dtype, void *stream);
+
+/*
+ * Gradients of tllm_qk_norm_rope at q and k, given those of its outputs (dq_out, dk_out): dq, dk,
+ * and dwq, dwk [D] (contiguous, the I/O dtype; summed in fp32 in a fixed order). workspace:
+ * tllm_qk_norm_rope_bwd_workspace_size bytes, 16-byte aligned.
+ */
+TLLM_API size_t tllm_qk_norm_rope_bwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D);
+TLLM_API int tllm_qk_norm_rope_bwd(const void *dq_out, const void *dk_out, const void *q,
+                                   const void *k, const void *wq, const void *wk, const float *cos,
+                                   const float *sin, const int32_t *positions, void *dq, void *dk,
+                                   void *dwq, void *dwk, void *workspace, size_t workspace_bytes,
+                                   int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rope_rows,
+                                   int64_t scos, int64_t ssin, int64_t axes, int64_t spos,
+                                   const uint32_t *axis_of_pair, const int64_t *sdqo,
+                                   const int64_t *sdko, const int64_t *sq, const int64_t *sk,
+                                   const int64_t *sdq, const int64_t *sdk, float eps, int dtype,
+                                   void *stream);
+
+/*
+ * The 4-bit paged KV cache (no counterpart in the reference, whose cache is fp16 or bf16:
+ * python/triton_llm/ops/paged_attention.py:92-128). cache is uint8 [num_blocks, Hkv,
+ * block_size / 16, 20 * D]: 16 tokens of one head per row, K then V (tritonllmcompiler_b200/csrc/
+ * kv4.cuh has the order inside a row). Strides sc are {block, head} in bytes, multiples of 16, the
+ * rows of a block and head contiguous; D 64 or 128, block_size 16, 32 or 64. Each group of 32
+ * channels x of a token and head holds scale s = fp16((max - min) / 15) and zero z = fp16(min), and
+ * codes c = clamp(rint((x - z) / s), 0, 15), 0 where s is 0; it stands for c * s + z.
+ *
+ * tllm_paged_kv4_append quantises k and v [T, Hkv, D] (strides sk/sv {token, head}) into slots
+ * [T] (block * block_size + offset; negative: skipped; past the pool: skipped and reported through
+ * tllm_debug_status). tllm_paged_kv4_gather writes the values that slots hold into k and v (zeros
+ * for slots that hold nothing).
+ */
+TLLM_API int tllm_paged_kv4_append(const void *k, const void *v, void *cache, const int32_t *slots,
+                                   int64_t T, int64_t Hkv, int64_t D, int64_t block_size,
+                                   int64_t num_blocks, const int64_t *sk, const int64_t *sv,
+                                   const int64_t *sc, int dtype, void *stream);
+TLLM_API int tllm_paged_kv4_gather(const void *cache, const int32_t *slots, void *k, void *v,
+                                   int64_t T, int64_t Hkv, int64_t D, int64_t block_size,
+                                   int64_t num_blocks, const int64_t *sk, const int64_t *sv,
+                                   const int64_t *sc, int dtype, void *stream);
+
+/*
+ * Attention of packed new tokens over the 4-bit paged cache: q and o [T, Hq, D] (strides sq/so
+ * {token, head}, multiples of 8 elements), Hq % Hkv == 0, query head h reading KV head
+ * h / (Hq / Hkv). Sequence b owns rows cu_seqlens[b] .. cu_seqlens[b + 1] (at most max_new), its
+ * newest tokens, already in the cache and counted by context_lens[b]; with causal != 0 a token
+ * sees the keys up to its own position, else all of them. Rows that see no key give NaN; rows
+ * past cu_seqlens[B] give zeros. Block-table entries outside the pool read block 0 and are
+ * reported through tllm_debug_status. workspace: tllm_paged_kv4_attn_workspace_size bytes,
+ * 256-byte aligned (0 when no launch splits the keys).
+ */
+TLLM_API size_t tllm_paged_kv4_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                                   int64_t max_new, int64_t D, int64_t block_size,
+                                                   int64_t max_blocks);
+TLLM_API int tllm_paged_kv4_attn(const void *q, const void *cache, const int32_t *block_tables,
+                                 const int32_t *context_lens, const int32_t *cu_seqlens, void *o,
+                                 void *workspace, size_t workspace_bytes, int64_t B, int64_t T,
+                                 int64_t Hq, int64_t Hkv, int64_t max_new, int64_t D,
+                                 int64_t block_size, int64_t max_blocks, int64_t num_blocks,
+                                 const int64_t *sq, const int64_t *sc, const int64_t *sbt,
+                                 const int64_t *so, float sm_scale, int causal, int dtype,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

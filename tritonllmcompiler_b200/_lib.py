@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libtllm_sm1
 DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
 
 _c_i64p = ctypes.POINTER(ctypes.c_int64)
+_c_u32p = ctypes.POINTER(ctypes.c_uint32)
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 
@@ -130,6 +131,41 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, _vp],
+    ),
+    "tllm_paged_plan": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _c_i64p, _vp],
+    ),
+    "tllm_qk_norm_rope": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _c_u32p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int,
+         _vp],
+    ),
+    "tllm_qk_norm_rope_bwd_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
+    "tllm_qk_norm_rope_bwd": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_u32p, _c_i64p, _c_i64p, _c_i64p,
+         _c_i64p, _c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int, _vp],
+    ),
+    "tllm_paged_kv4_append": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _c_i64p, _c_i64p, _c_i64p,
+         ctypes.c_int, _vp],
+    ),
+    "tllm_paged_kv4_gather": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _c_i64p, _c_i64p, _c_i64p,
+         ctypes.c_int, _vp],
+    ),
+    "tllm_paged_kv4_attn_workspace_size": (
+        ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "tllm_paged_kv4_attn": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _c_i64p, _c_i64p, _c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int,
+         ctypes.c_int, _vp],
     ),
     "tllm_swiglu_variant": (
         ctypes.c_int,

@@ -208,6 +208,9 @@ int ppf_read_status(int *out);
 int fbwd_read_status(int *out);
 int swiglu8_read_status(int *out);
 int qkv_read_status(int *out);
+int qknr_read_status(int *out);
+int kv4_read_status(int *out);
+int kv4a_read_status(int *out);
 namespace paged {
 int read_status(int *out);
 }
@@ -215,7 +218,8 @@ int read_status(int *out);
 int read_and_clear_device_status(int *out) {
   int (*readers[])(int *) = {flash_read_status, swiglu_read_status, paged::read_status,
                              selftest_read_status, pkv_read_status, ppf_read_status,
-                             fbwd_read_status, swiglu8_read_status, qkv_read_status};
+                             fbwd_read_status, swiglu8_read_status, qkv_read_status,
+                             qknr_read_status, kv4_read_status, kv4a_read_status};
   int first = 0;
   for (auto rd : readers) {
     int v = 0;
