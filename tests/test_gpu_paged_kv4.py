@@ -230,14 +230,15 @@ def test_rows_past_the_batch_are_zero(cuda_device, new):
     assert (none == 0).all()
 
 
-@pytest.mark.parametrize("new", [[4, 1], [40, 1]])
-def test_nan_keys_behind_the_mask(cuda_device, new):
-    """A NaN or an infinity in the newest token reaches only the rows that see it."""
-    lens, G = [90, 33], 4
+@pytest.mark.parametrize("lens,new", [([90, 33], [4, 1]), ([97, 33], [1, 1]), ([90, 33], [40, 1])])
+def test_nan_keys_behind_the_mask(cuda_device, lens, new):
+    """A NaN or an infinity in the newest token reaches the rows that see it (also where it is alone
+    in its tile) and no others."""
+    G, last = 4, lens[0] - 1
     q, cache, table, ctx, cu, k, v = _case(8, lens, new, 1, G, 128, 16, F)
     args = (table.cuda(), ctx.cuda(), cu.cuda(), max(new))
     ref = paged_attention_kv4(q.cuda(), cache, *args, block_size=16)
-    slot = (table[0, 89 // 16] * 16 + 89 % 16).view(1).cuda()
+    slot = (table[0, last // 16] * 16 + last % 16).view(1).cuda()
     bad = torch.full((1, 1, 128), float("nan"), dtype=F, device="cuda")
     bad[0, 0, 64:] = float("inf")
     paged_kv4_append(bad, bad, cache, slot, block_size=16)

@@ -37,27 +37,37 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 32;   // tokens a warp takes at a time: two pieces
 constexpr int kStages = 2;  // tiles of a warp in shared memory
+constexpr int kMinTiles = 2;  // a warp's least run of tiles
 
 enum : int { SITE_TILE = 0x41 };
+
+// A row tile of several workers: rows [r0, r0 + nr) of the sequence that starts at row0.
+struct __align__(16) Open {
+  int workers, slot, hk, row0;  // workers 0: none; the first part's slot
+  int r0, nr, pad0, pad1;
+};
 
 struct Args {
   const void *q;
   const uint8_t *cache;
   const int32_t *block_tables, *lens, *cu;
   void *o;
-  float *ws_ml;   // [row tiles][splits][rows of a tile][2] (maximum in log2 units, sum)
-  float *ws_acc;  // [row tiles][splits][rows of a tile][D]
+  // Partial results: two slots per worker (its first segment, its last), and per worker the row tile
+  // that starts in its last segment and goes on in the next workers.
+  Open *ws_open;    // [workers]
+  float2 *ws_ml;    // [slots][rows of a tile]: reference in log2 units, sum
+  float *ws_acc;    // [slots][rows of a tile][D]
   int64_t sq0, sq1, so0, so1, sblk, shead, sbt0, sbt1;
   int64_t T, num_blocks, max_blocks;
   int B, Hkv, G, log2_bs, causal, max_new;
-  int n_rt, splits, chunk;  // row tiles per sequence and KV head; key splits and their tokens
+  int n_rt, workers;  // row tiles per sequence and KV head; warps that share the tiles
   float scale_log2;
 };
 
-// Where a CTA works: sequence b, row tile rt (rows r0 .. r0 + nr of the n_q * G rows, row r being new
-// token r / G of query head hk * G + r % G), and how many keys its rows see.
+// A row tile: rows r0 .. r0 + nr of the n_q * G rows of sequence b and a KV head hk, row r being new
+// token r / G of query head hk * G + r % G, and how many keys they see.
 struct Place {
-  int b, rt, hk, r0, nr, row0, n_q, len, seen;
+  int b, rt, r0, nr, row0, n_q, len, seen;
 };
 
 __device__ __forceinline__ int row_keys(const Args &a, const Place &p, int r) {
@@ -65,10 +75,9 @@ __device__ __forceinline__ int row_keys(const Args &a, const Place &p, int r) {
 }
 
 template <int ROWS>
-__device__ __forceinline__ bool locate(const Args &a, int b, int rt, int hk, Place &p) {
+__device__ __forceinline__ bool locate(const Args &a, int b, int rt, Place &p) {
   p.b = b;
   p.rt = rt;
-  p.hk = hk;
   const int lim = static_cast<int>(a.T);
   p.row0 = min(max(__ldg(a.cu + b), 0), lim);
   p.n_q = min(max(__ldg(a.cu + b + 1), p.row0), lim) - p.row0;
@@ -98,11 +107,41 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // Transposes an 8 x 8 matrix of 16-bit values held as an MMA fragment.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b) { return Pack2<__half>::pack(a, b); }
+
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// All ones in the halves of v that are +0 (as the weights of hidden tokens are).
+__device__ __forceinline__ uint32_t zero_halves(uint32_t v) { return __vcmpeq2(v, 0u); }
+
+// v[r % W] without an indexed register.
+template <int W>
+__device__ __forceinline__ uint32_t pick(const uint32_t (&v)[W], int r) {
+  if constexpr (W == 2) return (r & 1) ? v[1] : v[0];
+  else return (r & 2) ? ((r & 1) ? v[3] : v[2]) : ((r & 1) ? v[1] : v[0]);
+}
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
@@ -120,35 +159,30 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {
   }
 }
 
-// The W fp16 scales of one token as fp32.
-template <int W>
-__device__ __forceinline__ void lds_scales(const uint8_t *p, float (&s)[W]) {
-  uint32_t w[W / 2];
-  lds_words<W / 2>(p, w);
-#pragma unroll
-  for (int i = 0; i < W / 2; ++i) {
-    const float2 f = Pack2<__half>::unpack(w[i]);
-    s[2 * i] = f.x;
-    s[2 * i + 1] = f.y;
-  }
-}
-
 // Four fp16 pairs from a word of two times four codes: x[0], x[2] are the codes of bits 0-3 and 8-11 of
 // each half times 2^-24, x[1], x[3] those of bits 4-7 and 12-15 times 2^-20 (subnormal numbers: the
 // codes' own bits, exact, without a conversion).
 __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
   x[0] = w & 0x000f000fu;
   x[1] = w & 0x00f000f0u;
-  w >>= 8;
-  x[2] = w & 0x000f000fu;
+  w = __byte_perm(w, 0u, 0x4341);  // the upper bytes of the halves
   x[3] = w & 0x00f000f0u;
+  x[2] = sub_half2(w, x[3]);  // exact, and not on the logic pipe, which is the busier one
 }
 
-// Few query rows per KV head (decode, speculative tokens): ROWS = 8 * NT rows a CTA.
+// Key tiles of a row tile; one where its rows see nothing, so that somebody writes them.
+__device__ __forceinline__ int key_tiles(const Place &p) { return max((p.seen + kTile - 1) / kTile, 1); }
+
+// Few query rows per KV head (decode, speculative tokens): ROWS = 8 * NT rows a row tile.
 //
-// A CTA takes `chunk` tokens of one sequence and KV head; its four warps take tiles of 32 tokens in
-// turn, each with its own ring of bulk copies (a page's K and V of one head are contiguous), its own
-// running maximum and sum, and no barrier until they are added up at the end.
+// All key tiles of all row tiles form one line: sequences, in them row tiles, in them KV heads, in
+// them tiles of 32 keys. Every warp of the grid, one wave of CTAs, takes an equal run of it (within a
+// tile), whatever the lengths are; each CTA finds its place by a scan over the sequences. A warp
+// works by itself: its own ring of bulk copies (a page's K and V of one head are contiguous), its
+// own running maximum and sum. A row tile that lies whole in a run is stored at once; otherwise each warp
+// stores its part, and kv4_merge_kernel adds the parts up. (CTAs of one row tile and 1024 keys
+// each, as before, spent 5 us of latency per CTA in starting and joining: 115 against @A us for 64
+// requests of U[512, 8192], 32 heads over 8.)
 //
 // Both products run as 16 x 8 x 16 MMAs with the cache as the 16-row operand, so 8 query rows fill
 // them: S^T = K Q^T and O^T = V^T P^T. The operands from the cache are the codes themselves, as fp16
@@ -156,66 +190,127 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 // cheap:
 //   q . k = sum_g s_g (sum_{d in g} q_d c_d) + sum_g z_g (sum_{d in g} q_d): one FMA per group and
 //           score on the products' fp32 results; the zeros are one more MMA with the sums of q, held as
-//           high and low fp16 parts;
-//   o_d   = sum_t (p_t s_{t,g}) c_{t,d} + sum_t p_t z_{t,g}: the weights times the scales are rounded
-//           to fp16 per group, after a common power of two (from the largest scale met so far) that
-//           keeps them in fp16's normal range; the zeros are one more MMA with 16 x 8 results.
-// q is brought to [2^9, 2^10) by a power of two per row and is exact in fp16 from either type.
+//           high and low fp16 parts. q is brought to [2^12, 2^13) by a power of two per row and is
+//           exact in fp16 from either type, so scores are exact but for fp32 sums.
+//   o_d   = sum_t (p_t s_{t,g}) (c_{t,d} - 8) + sum_t p_t (z_{t,g} + 8 s_{t,g}): weights are fp16, and
+//           fp16 again after the scale (packed products on the transposed weights, a third of the
+//           instructions of fp32 ones), so their rounding errors meet values centred on 0 in
+//           both sums: without the 8 they would meet values of twice that size that cancel. The 8 is
+//           one MMA with a constant operand for each of the codes'. The second sum is an MMA.
+// Weights are 2^(x - mu) with mu = m - k: k <= 12 keeps the weights times the scales in fp16's normal
+// range whatever the size of V (from the largest scale met), and m follows the maximum only
+// when it grows by more than 2^3 (weights and products stay under 2^15).
 // An S^T result becomes a P^T operand by transposing 8 x 8 blocks in registers (movmatrix).
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
   using P = Piece<D>;
   constexpr int W = P::W;
   constexpr int ROWS = 8 * NT;
   constexpr int TILE_BYTES = 2 * P::BYTES;
-  constexpr int RING = kStages * TILE_BYTES;
-  static_assert(RING >= ROWS * D * 4, "a warp's results reuse its ring");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[kWarps][kStages];
-  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
-  __shared__ int s_abort;
+  __shared__ int64_t s_scan[kWarps], s_off[kWarps];
+  __shared__ int s_seq[kWarps], s_abort;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, cq = lane & 3;  // fragment row (token, channel or query row) and column pair
-
-  // ---- place ----
-  const int64_t main_ctas = static_cast<int64_t>(a.B) * a.n_rt * a.splits * a.Hkv;
-  if (blockIdx.x >= main_ctas) {  // the last CTA clears the rows that belong to no sequence
-    const int64_t from = a.B > 0 ? min(max(static_cast<int64_t>(__ldg(a.cu + a.B)), int64_t{0}), a.T) : 0;
-    const int64_t n = (a.T - from) * a.Hkv * a.G * (D / 8);
-    for (int64_t i = tid; i < n; i += kThreads) {
-      const int64_t row = i / (D / 8);
-      T *o = static_cast<T *>(a.o) + (from + row / (a.Hkv * a.G)) * a.so0 + (row % (a.Hkv * a.G)) * a.so1;
-      *reinterpret_cast<uint4 *>(o + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-    }
-    return;
-  }
-  const int idx = static_cast<int>(blockIdx.x);
-  const int hk = idx % a.Hkv;
-  const int split = idx / a.Hkv % a.splits;
-  const int brt = idx / a.Hkv / a.splits;
-  Place pl;
-  if (!locate<ROWS>(a, brt / a.n_rt, brt % a.n_rt, hk, pl)) return;
-  if (pl.n_q > a.max_new && tid == 0) atomicCAS(&g_kv4a_status, 0, TLLM_DEV_BAD_INDEX);
-  const int t0 = split * a.chunk;
-  const int n = max(min(pl.seen - t0, a.chunk), 0);
-  if (n == 0 && split > 0) return;  // the merge knows; split 0 always runs, for rows without keys
-  const int n_tiles = (n + kTile - 1) / kTile;
-  const int nk = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;  // this warp's tiles
 
   if (tid == 0) {
     for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_u32(&s_bar[0][0] + i), 1);
     s_abort = 0;
     fence_mbar_init();
   }
-  __syncthreads();
 
-  // ---- the warp's ring: tile k is tile warp + kWarps * k of the chunk ----
-  uint8_t *ring = smem + warp * RING;
-  int page0 = 0, page1 = 0;  // lane l: pages of tile 32 i + l
-  auto issue = [&](int k) {
+  // ---- the line and this warp's run of it ----
+  const int worker = blockIdx.x * kWarps + warp;
+  const int share = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
+  auto tiles_of_seq = [&](int b) {
+    int64_t t = 0;
+    Place p;
+    for (int rt = 0; rt < a.n_rt && locate<ROWS>(a, b, rt, p); ++rt) t += key_tiles(p);
+    if (p.n_q > a.max_new) atomicCAS(&g_kv4a_status, 0, TLLM_DEV_BAD_INDEX);
+    return t * a.Hkv;
+  };
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of_seq(b);
+  int64_t upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += u;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += s_scan[w];
+    total += s_scan[w];
+  }
+  const int64_t per = max((total + a.workers - 1) / a.workers, static_cast<int64_t>(kMinTiles));
+  for (int w = 0; w < kWarps; ++w) {
+    int64_t off = (static_cast<int64_t>(blockIdx.x) * kWarps + w) * per - (upto - mine);
+    if (off < 0 || off >= mine) continue;
+    for (int b = b0; b < b1; ++b) {
+      const int64_t t = tiles_of_seq(b);
+      if (off < t) {
+        s_seq[w] = b;
+        s_off[w] = off;
+        break;
+      }
+      off -= t;
+    }
+  }
+  // Rows that belong to no sequence are cleared.
+  {
+    const int64_t from = a.B > 0 ? min(max(static_cast<int64_t>(__ldg(a.cu + a.B)), int64_t{0}), a.T) : 0;
+    const int hq = a.Hkv * a.G;
+    const int64_t n = (a.T - from) * hq * (D / 8);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < n; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+      const int64_t row = i / (D / 8);
+      T *o = static_cast<T *>(a.o) + (from + row / hq) * a.so0 + (row % hq) * a.so1;
+      *reinterpret_cast<uint4 *>(o + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __syncthreads();
+  if (lane == 0) a.ws_open[worker].workers = 0;
+  int64_t pos = worker * per;
+  const int64_t end = min(pos + per, total);
+  if (pos >= end) return;
+  Place pl;
+  int nt, hk, first;  // the segment's row tile has nt key tiles; the segment starts at `first`
+  {
+    int64_t off = s_off[warp];
+    int b = s_seq[warp], rt = 0;
+    while (b < a.B) {  // (always found: pos < total)
+      if (locate<ROWS>(a, b, rt, pl)) {
+        nt = key_tiles(pl);
+        if (off < static_cast<int64_t>(nt) * a.Hkv) break;
+        off -= static_cast<int64_t>(nt) * a.Hkv;
+      }
+      if (++rt == a.n_rt) {
+        rt = 0;
+        ++b;
+      }
+    }
+    if (b == a.B) return;
+    hk = static_cast<int>(off / nt);
+    first = static_cast<int>(off % nt);
+  }
+  int count = static_cast<int>(min(static_cast<int64_t>(nt - first), end - pos));
+  bool at_start = true;  // the worker's first segment
+
+  // ---- the warp's ring ----
+  uint8_t *ring = smem + warp * (kStages * TILE_BYTES);
+  // This warp's fragments of q, kept out of the registers: [row tile of 8][word][lane].
+  uint4 *qf = reinterpret_cast<uint4 *>(smem + kWarps * kStages * TILE_BYTES) + warp * (NT * W * 32);
+  uint32_t taken = 0;        // tiles taken from the ring so far, over all segments
+  int page0 = 0, page1 = 0;  // lane l: pages of the segment's tile 32 i + l
+  // Starts the copy of the segment's tile k, `ahead` tiles after the next one to be taken.
+  auto issue = [&](int k, int ahead) {
     if ((k & 31) == 0) {
-      const int tok = t0 + (warp + kWarps * (k + lane)) * kTile;
+      const int tok = (first + k + lane) * kTile;
       auto page = [&](int t) -> int {
         if (t >= pl.seen) return 0;
         const int p = __ldg(a.block_tables + pl.b * a.sbt0 + (t >> a.log2_bs) * a.sbt1);
@@ -223,36 +318,37 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
         atomicCAS(&g_kv4a_status, 0, TLLM_DEV_BAD_INDEX);
         return 0;
       };
-      if (k + lane < nk) {
+      if (k + lane < count) {
         page0 = page(tok);
-        page1 = a.log2_bs == 4 ? page(tok + kPieceTokens) : page0;
+        if (a.log2_bs == 4) page1 = page(tok + kPieceTokens);
       }
     }
-    const int64_t p0 = __shfl_sync(0xffffffffu, page0, k & 31);
-    const int64_t p1 = __shfl_sync(0xffffffffu, page1, k & 31);
-    if (lane == 0) {
-      const int at = (warp + kWarps * k) * kTile;
-      const bool both = n - at > kPieceTokens;
-      const uint32_t bar = smem_u32(&s_bar[warp][k % kStages]);
-      const uint32_t dst = smem_u32(ring + (k % kStages) * TILE_BYTES);
-      const uint8_t *head = a.cache + hk * a.shead;
+    if (lane == (k & 31)) {  // the lane that has the pages
+      const int tok = (first + k) * kTile;
+      const bool both = pl.seen - tok > kPieceTokens;
+      const uint32_t stage = (taken + ahead) % kStages;
+      const uint32_t bar = smem_u32(&s_bar[warp][stage]), dst = smem_u32(ring) + stage * TILE_BYTES;
+      const uint8_t *src = a.cache + hk * a.shead + page0 * a.sblk;
       mbar_arrive_expect_tx(bar, both ? TILE_BYTES : P::BYTES);
       if (a.log2_bs == 4) {
-        bulk_load(dst, head + p0 * a.sblk, P::BYTES, bar);
-        if (both) bulk_load(dst + P::BYTES, head + p1 * a.sblk, P::BYTES, bar);
+        bulk_load(dst, src, P::BYTES, bar);
+        if (both) bulk_load(dst + P::BYTES, a.cache + hk * a.shead + page1 * a.sblk, P::BYTES, bar);
       } else {
-        const int piece = ((t0 + at) & ((1 << a.log2_bs) - 1)) / kPieceTokens;
-        bulk_load(dst, head + p0 * a.sblk + piece * P::BYTES, both ? TILE_BYTES : P::BYTES, bar);
+        const int piece = (tok & ((1 << a.log2_bs) - 1)) / kPieceTokens;
+        bulk_load(dst, src + piece * P::BYTES, both ? TILE_BYTES : P::BYTES, bar);
       }
     }
   };
-  for (int k = 0; k < kStages && k < nk; ++k) issue(k);
+  auto prime = [&] {
+    for (int k = 0; k < kStages && k < count && pl.seen > 0; ++k) issue(k, k);
+  };
+  prime();
 
+  while (true) {
   // ---- q: B fragments of Q^T, and each row's sums over the groups ----
-  uint32_t qb[NT][W][4];  // words w: pairs {0,1}, {2,3} 2^-4, {4,5}, {6,7} 2^-4 of channels 32 w + 8 cq
   uint32_t qs[NT];
-  float rs[NT][2];  // score factor of query rows 8 j + 2 cq, + 1
-  int lim[NT][2];   // keys (from t0) that they see
+  float rs[NT][2];  // score factor (log2 units) of query rows 8 j + 2 cq, + 1
+  int lim[NT][2];   // keys that they see
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int row = pl.r0 + 8 * j + r;
@@ -275,9 +371,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // An infinite row keeps its infinities; a zero or subnormal one is scaled by 2^109 at most.
+    // An infinite row keeps its infinities; a zero or subnormal one is scaled by 2^112 at most.
     const int e = max((__float_as_int(top) >> 23) - 127, -100);
-    const float up = pow2(9 - e);
+    const float up = pow2(12 - e);
     float hi[W], lo[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -289,12 +385,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= pow2(-24);  // the codes' unit; |sum| < 2^-6
       hi[w] = __half2float(__float2half_rn(sum));
       lo[w] = sum - hi[w];
-      qb[j][w][0] = pack_half(f[w][0], f[w][1]);
-      qb[j][w][1] = pack_half(f[w][2] * 0.0625f, f[w][3] * 0.0625f);
-      qb[j][w][2] = pack_half(f[w][4], f[w][5]);
-      qb[j][w][3] = pack_half(f[w][6] * 0.0625f, f[w][7] * 0.0625f);
+      // pairs {0,1}, {2,3} 2^-4, {4,5}, {6,7} 2^-4 of channels 32 w + 8 cq
+      qf[(j * W + w) * 32 + lane] =
+          make_uint4(pack_half(f[w][0], f[w][1]), pack_half(f[w][2] * 0.0625f, f[w][3] * 0.0625f),
+                     pack_half(f[w][4], f[w][5]), pack_half(f[w][6] * 0.0625f, f[w][7] * 0.0625f));
     }
     // K index of the zeros' MMA: group g of the high parts, then of the low ones.
     qs[j] = 0;
@@ -303,19 +400,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
       if (cq == i / 2) qs[j] = pack_half(hi[i], hi[i + 1]);
       if (cq == W / 2 + i / 2) qs[j] = pack_half(lo[i], lo[i + 1]);
     }
-    const float down = pow2(e - 9) * a.scale_log2;
+    const float down = pow2(e) * (4096.f * a.scale_log2);  // 2^(e - 12) for q, 2^24 for the codes' unit
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       rs[j][c] = __shfl_sync(0xffffffffu, down, 4 * (2 * cq + c));
       const int rr = 8 * j + 2 * cq + c;
-      lim[j][c] = rr < pl.nr ? row_keys(a, pl, pl.r0 + rr) - t0 : n;
+      lim[j][c] = rr < pl.nr ? row_keys(a, pl, pl.r0 + rr) : pl.seen;
     }
   }
-  const int lim_all = min(row_keys(a, pl, pl.r0) - t0, n);  // below this every row sees every key
+  const int lim_all = row_keys(a, pl, pl.r0);  // below this every row sees every key
 
   float acc[W][2][NT][4];  // O^T: [group][half][row tile]: channels 32 g + 4 r + 2 half (+ 1 in 2, 3)
   float accz[NT][4];       // zeros: row g of lane group r = g
-  float m[NT][2], l[NT][2];
+  float m[NT][2], mu[NT][2], l[NT][2];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -325,73 +422,64 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
       for (int g = 0; g < W; ++g) acc[g][0][j][i] = acc[g][1][j][i] = 0.f;
     }
     m[j][0] = m[j][1] = -INFINITY;
-    l[j][0] = l[j][1] = 0.f;
+    mu[j][0] = mu[j][1] = l[j][0] = l[j][1] = 0.f;
   }
   int v_exp = 0;  // exponent field of the largest V scale so far
-
-  auto scale_acc = [&](const float (&f)[NT][2]) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int g = 0; g < W; ++g) {
-          acc[g][0][j][i] *= f[j][i & 1];
-          acc[g][1][j][i] *= f[j][i & 1];
-        }
-  };
 
   // One tile. kMask: some row does not see all of its 32 tokens.
   auto tile = [&](uint8_t *base, int at, auto mask_tag) {
     constexpr bool kMask = decltype(mask_tag)::value;
     if constexpr (kMask) {
-      // Slots past the last key may hold anything: their V scales and zeros become 0. A zero that is
-      // no number, in a token that only some rows see, would reach every row through its MMA; its
-      // scale is then no number either, and alone marks the rows that do see it.
-      uint8_t *pb = base + (lane >> 4) * P::BYTES;
-      const int tok = lane & 15;
-      const bool past = at + lane >= n;
+      // Slots past the last key may hold anything: their V scales and zeros become 0.
+      if (at + lane >= pl.seen) {
+        uint8_t *pb = base + (lane >> 4) * P::BYTES;
 #pragma unroll
-      for (int g = 0; g < W; ++g) {
-        uint16_t *z = reinterpret_cast<uint16_t *>(pb + P::v_zero(tok, g));
-        if (past) *reinterpret_cast<uint16_t *>(pb + P::v_scale(tok, g)) = 0;
-        if (past || (*z & 0x7c00u) == 0x7c00u) *z = 0;
+        for (int g = 0; g < W; ++g) {
+          *reinterpret_cast<uint16_t *>(pb + P::v_scale(lane & 15, g)) = 0;
+          *reinterpret_cast<uint16_t *>(pb + P::v_zero(lane & 15, g)) = 0;
+        }
       }
       __syncwarp();
     }
     // ---- scores ----
     float x[2][NT][4];
+    uint32_t k0[2][W], k1[2][W], s0[2][W / 2], s1[2][W / 2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint8_t *pb = base + h * P::BYTES;
+      lds_words<W>(pb + P::K_CODES + r * (D / 2) + cq * (4 * W), k0[h]);
+      lds_words<W>(pb + P::K_CODES + (r + 8) * (D / 2) + cq * (4 * W), k1[h]);
+      lds_words<W / 2>(pb + P::k_scale(r, 0), s0[h]);
+      lds_words<W / 2>(pb + P::k_scale(r + 8, 0), s1[h]);
       uint32_t z0 = 0, z1 = 0;
       if (W == 4 || cq < 2) {
         const uint8_t *zp = pb + P::k_zero(r, 0) + 4 * (cq % (W / 2));
         z0 = *reinterpret_cast<const uint32_t *>(zp);
         z1 = *reinterpret_cast<const uint32_t *>(zp + 8 * 2 * W);
       }
-      uint32_t k0[W], k1[W];
-      lds_words<W>(pb + P::K_CODES + r * (D / 2) + cq * (4 * W), k0);
-      lds_words<W>(pb + P::K_CODES + (r + 8) * (D / 2) + cq * (4 * W), k1);
-      float s0[W], s1[W];
-      lds_scales<W>(pb + P::k_scale(r, 0), s0);
-      lds_scales<W>(pb + P::k_scale(r + 8, 0), s1);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         x[h][j][0] = x[h][j][1] = x[h][j][2] = x[h][j][3] = 0.f;
         mma16816(x[h][j], z0, z1, 0u, 0u, qs[j], 0u);
       }
+    }
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < W; ++w) {
+      uint4 qb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) qb[j] = qf[(j * W + w) * 32 + lane];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         uint32_t u0[4], u1[4];
-        spread(k0[w], u0);
-        spread(k1[w], u1);
-        const float f0 = s0[w] * 16777216.f, f1 = s1[w] * 16777216.f;
+        spread(k0[h][w], u0);
+        spread(k1[h][w], u1);
+        const float2 p0 = Pack2<__half>::unpack(s0[h][w / 2]), p1 = Pack2<__half>::unpack(s1[h][w / 2]);
+        const float f0 = (w & 1) ? p0.y : p0.x, f1 = (w & 1) ? p1.y : p1.x;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float c[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816(c, u0[0], u1[0], u0[1], u1[1], qb[j][w][0], qb[j][w][1]);
-          mma16816(c, u0[2], u1[2], u0[3], u1[3], qb[j][w][2], qb[j][w][3]);
+          mma16816(c, u0[0], u1[0], u0[1], u1[1], qb[j].x, qb[j].y);
+          mma16816(c, u0[2], u1[2], u0[3], u1[3], qb[j].z, qb[j].w);
           x[h][j][0] = fmaf(f0, c[0], x[h][j][0]);
           x[h][j][1] = fmaf(f0, c[1], x[h][j][1]);
           x[h][j][2] = fmaf(f1, c[2], x[h][j][2]);
@@ -399,95 +487,102 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
         }
       }
     }
-    // ---- softmax: a lane has tokens r, r + 8 of each piece for rows 2 cq, 2 cq + 1 ----
-    float m2[NT][2];
+    // ---- references: a lane has tokens r, r + 8 of each piece for rows 2 cq, 2 cq + 1 ----
     bool grew = false;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = m[j][c];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float &v = x[h][j][c + 2 * i];
-            v *= rs[j][c];
+            x[h][j][c + 2 * i] *= rs[j][c];
             if constexpr (kMask)
-              if (at + 16 * h + r + 8 * i >= lim[j][c]) v = -INFINITY;
-            top = fmaxf(top, v);
+              if (at + 16 * h + r + 8 * i >= lim[j][c]) x[h][j][c + 2 * i] = -INFINITY;
           }
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        m2[j][c] = top;
-        grew |= top > m[j][c];
+        grew |= fmaxf(fmaxf(x[0][j][c], x[0][j][c + 2]), fmaxf(x[1][j][c], x[1][j][c + 2])) > m[j][c];
       }
-    if (__any_sync(0xffffffffu, grew)) {
-      float f[NT][2];
+    int e;  // exponent field of the tile's largest V scale
+    {
+      uint32_t v[W / 2], big = 0;
+      lds_words<W / 2>(base + (lane >> 4) * P::BYTES + P::V_SCALE + (lane & 15) * 2 * W, v);
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) big = __vmaxu2(big, v[i] & 0x7fff7fffu);
+      e = static_cast<int>(__reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16)) >> 10);
+      if (e == 31) {  // infinities and NaNs do not count
+        big = 0;
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+          const uint32_t u = v[i] & 0x7fff7fffu;
+          big = __vmaxu2(big, u & __vcmpltu2(u, 0x7c007c00u));
+        }
+        e = static_cast<int>(__reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16)) >> 10);
+      }
+    }
+    if (__any_sync(0xffffffffu, grew) || e > v_exp) {
+      v_exp = max(v_exp, e);
+      const float shift = static_cast<float>(min(12, 26 - v_exp));
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          f[j][c] = m[j][c] == -INFINITY ? 1.f : ex2_approx(m[j][c] - m2[j][c]);  // 1: nothing summed yet
-          m[j][c] = m2[j][c];
-          l[j][c] *= f[j][c];
-          accz[j][c] *= f[j][c];
-          accz[j][c + 2] *= f[j][c];
+          float top = fmaxf(fmaxf(x[0][j][c], x[0][j][c + 2]), fmaxf(x[1][j][c], x[1][j][c + 2]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          // m is the reference's maximum and the 2^3 that a weight may grow beyond it.
+          const bool had = m[j][c] != -INFINITY;
+          if (top > m[j][c]) m[j][c] = top + 3.f;
+          const float to = m[j][c] == -INFINITY ? 0.f : m[j][c] - 3.f - shift;
+          const float f = had ? ex2_approx(mu[j][c] - to) : 1.f;
+          mu[j][c] = to;
+          l[j][c] *= f;
+          accz[j][c] *= f;
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
+            acc[g][0][j][c] *= f;
+            acc[g][0][j][c + 2] *= f;
+            acc[g][1][j][c] *= f;
+            acc[g][1][j][c + 2] *= f;
+          }
         }
-      scale_acc(f);
     }
-    // ---- the largest V scale of the tile ----
-    {
-      uint32_t v[W / 2], top = 0;
-      lds_words<W / 2>(base + (lane >> 4) * P::BYTES + P::V_SCALE + (lane & 15) * 2 * W, v);
-#pragma unroll
-      for (int i = 0; i < W / 2; ++i) {
-        const uint32_t u = v[i] & 0x7fff7fffu;
-        top = __vmaxu2(top, u & __vcmpltu2(u, 0x7c007c00u));  // infinities and NaNs do not count
-      }
-      top = max(top & 0xffffu, top >> 16) >> 10;
-      const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, top));  // 0 .. 30
-      if (e > v_exp) {
-        float f[NT][2];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) f[j][0] = f[j][1] = pow2(v_exp - e);
-        scale_acc(f);
-        v_exp = e;
-      }
-    }
-    const float up = pow2(23 - v_exp);  // weight times scale times up < 2^9
     // ---- weights and O^T ----
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint8_t *pb = base + h * P::BYTES;
-      float s0[W], s1[W];
-      lds_scales<W>(pb + P::v_scale(r, 0), s0);
-      lds_scales<W>(pb + P::v_scale(r + 8, 0), s1);
-      uint32_t z0 = 0, z2 = 0;
-      if (r < W) {
-        const uint8_t *zp = pb + P::v_zero(2 * cq, r);
-        z0 = *reinterpret_cast<const uint32_t *>(zp);
-        z2 = *reinterpret_cast<const uint32_t *>(zp + 16);
+      // Token pairs cq and cq + 4: scales of both tokens per group, zeros of group r % W, codes.
+      uint32_t sw[W], s0[W], s1[W];
+      lds_words<W>(pb + P::v_scale(2 * cq, 0), sw);
+#pragma unroll
+      for (int g = 0; g < W; ++g) s0[g] = __byte_perm(sw[g / 2], sw[W / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410);
+      lds_words<W>(pb + P::v_scale(2 * cq + 8, 0), sw);
+#pragma unroll
+      for (int g = 0; g < W; ++g) s1[g] = __byte_perm(sw[g / 2], sw[W / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410);
+      const uint8_t *zp = pb + P::v_zero(2 * cq, r % W);
+      uint32_t z0 = *reinterpret_cast<const uint32_t *>(zp), z1 = *reinterpret_cast<const uint32_t *>(zp + 16);
+      z0 = fma_half2(pick<W>(s0, r), 0x48004800u, z0);  // z + 8 s
+      z1 = fma_half2(pick<W>(s1, r), 0x48004800u, z1);
+      if constexpr (kMask) {  // no number: left to the rows that see the token (their weights say so)
+        z0 &= ~__vcmpeq2(z0 & 0x7c007c00u, 0x7c007c00u);
+        z1 &= ~__vcmpeq2(z1 & 0x7c007c00u, 0x7c007c00u);
       }
-      // Token pairs cq and cq + 4; W / 2 words of each token.
       const uint8_t *vp = pb + P::V_CODES + cq * D + (r ^ P::swizzle(cq)) * P::CHUNK;
       uint32_t v0[W], v1[W];
       lds_words<W>(vp, v0);
       lds_words<W>(vp + 4 * D, v1);
-      float pf[NT][4];
+      uint32_t b0[NT], b1[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
+        float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float mu = m[j][i & 1] == -INFINITY ? 0.f : m[j][i & 1];
-          pf[j][i] = ex2_approx(x[h][j][i] - mu);
-          l[j][i & 1] += pf[j][i];
+          p[i] = ex2_approx(x[h][j][i] - mu[j][i & 1]);
+          l[j][i & 1] += p[i];
         }
-        const uint32_t b0 = transpose8(pack_half(pf[j][0], pf[j][1]));
-        const uint32_t b1 = transpose8(pack_half(pf[j][2], pf[j][3]));
-        mma16816(accz[j], z0, 0u, z2, 0u, b0, b1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pf[j][i] *= up;
+        b0[j] = transpose8(pack_half(p[0], p[1]));
+        b1[j] = transpose8(pack_half(p[2], p[3]));
+        mma16816(accz[j], z0, 0u, z1, 0u, b0[j], b1[j]);
       }
 #pragma unroll
       for (int g = 0; g < W; ++g) {
@@ -496,31 +591,41 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
         spread(__byte_perm(v0[g / 2], v0[W / 2 + g / 2], sel), u0);
         spread(__byte_perm(v1[g / 2], v1[W / 2 + g / 2], sel), u1);
 #pragma unroll
+        for (int i = 0; i < 4; ++i) {  // -8 in the two units
+          u0[i] = add_half2(u0[i], (i & 1) ? 0x80808080u : 0x80088008u);
+          u1[i] = add_half2(u1[i], (i & 1) ? 0x80808080u : 0x80088008u);
+        }
+#pragma unroll
         for (int j = 0; j < NT; ++j) {
-          float w0 = pf[j][0] * s0[g], w1 = pf[j][1] * s0[g], w2 = pf[j][2] * s1[g], w3 = pf[j][3] * s1[g];
+          uint32_t w0 = mul_half2(b0[j], s0[g]), w1 = mul_half2(b1[j], s1[g]);
           if constexpr (kMask) {  // a hidden token's scale may be no number
-            if (pf[j][0] == 0.f) w0 = 0.f;
-            if (pf[j][1] == 0.f) w1 = 0.f;
-            if (pf[j][2] == 0.f) w2 = 0.f;
-            if (pf[j][3] == 0.f) w3 = 0.f;
+            w0 &= ~zero_halves(b0[j]);
+            w1 &= ~zero_halves(b1[j]);
           }
-          const uint32_t b0 = transpose8(pack_half(w0, w1));
-          const uint32_t b1 = transpose8(pack_half(w2, w3));
-          mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], b0, b1);
-          mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], b0, b1);
+          mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], w0, w1);
+          mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], w0, w1);
         }
       }
     }
   };
 
   bool ok = true;
-  int k = 0;
-  for (; k < nk && ok; ++k) {
-    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_bar[warp][k % kStages]), (k / kStages) & 1, &s_abort,
-                                           &g_kv4a_status, TLLM_DEV_WAIT_TIMEOUT + SITE_TILE));
-    if (!ok) break;
-    const int at = (warp + kWarps * k) * kTile;
-    uint8_t *base = ring + (k % kStages) * TILE_BYTES;
+  for (int k = 0; k < count && pl.seen > 0; ++k, ++taken) {
+    const uint32_t stage = taken % kStages, bar = smem_u32(&s_bar[warp][stage]), parity = (taken / kStages) & 1;
+    if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &s_abort, &g_kv4a_status, TLLM_DEV_WAIT_TIMEOUT + SITE_TILE));
+    if (!ok) {
+      // The copies in flight still write to this CTA's memory: give them their time, then leave.
+      for (int i = 0; i < kStages && k + i < count; ++i) {
+        const long long since = clock64();
+        while (!mbar_try_wait(smem_u32(&s_bar[warp][(taken + i) % kStages]), ((taken + i) / kStages) & 1) &&
+               clock64() - since < kWaitLimitCycles) {
+        }
+      }
+      return;
+    }
+    const int at = (first + k) * kTile;
+    uint8_t *base = ring + stage * TILE_BYTES;
     if (at + kTile > lim_all) {
       tile(base, at, std::true_type{});
       fence_proxy_async_smem();  // the tile was written to; a later copy may follow
@@ -528,19 +633,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
       tile(base, at, std::false_type{});
     }
     __syncwarp();
-    if (k + kStages < nk) issue(k + kStages);
-  }
-  // After a wait that gave up: the copies in flight still write to this CTA's memory.
-  for (int i = k; !ok && i < nk && i < k + kStages; ++i) {
-    const long long since = clock64();
-    while (!mbar_try_wait(smem_u32(&s_bar[warp][i % kStages]), (i / kStages) & 1) &&
-           clock64() - since < kWaitLimitCycles) {
-    }
+    if (k + kStages < count) issue(k + kStages, kStages);
   }
 
-  // ---- the warps' results, through their rings ----
-  const float f1 = pow2(1 + v_exp), f2 = pow2(v_exp - 3);  // 2^24 / up and 2^20 / up
-  float *mine = reinterpret_cast<float *>(ring);
+  // ---- this segment's results; the next one's copies go out first ----
+  const Place done = pl;
+  const int done_hk = hk, done_first = first, done_count = count, done_nt = nt;
+  const int64_t done_pos = pos;
+  pos += count;
+  const bool more = pos < end;
+  if (more) {
+    first = 0;
+    if (++hk == a.Hkv) {
+      hk = 0;
+      int b = pl.b, rt = pl.rt;
+      do {
+        if (++rt == a.n_rt) {
+          rt = 0;
+          ++b;
+        }
+      } while (b < a.B && !locate<ROWS>(a, b, rt, pl));
+      if (b == a.B) return;  // (always found: pos < total)
+      nt = key_tiles(pl);
+    }
+    count = static_cast<int>(min(static_cast<int64_t>(nt), end - pos));
+    prime();
+  }
+  const bool whole = done_count == done_nt;
+  const int64_t slot = 2 * static_cast<int64_t>(worker) + (at_start ? 0 : 1);
+  if (!whole && done_first == 0 && lane == 0)
+    a.ws_open[worker] = Open{static_cast<int>((done_pos + done_nt - 1) / per) - worker + 1, static_cast<int>(slot),
+                             done_hk, done.row0, done.r0, done.nr, 0, 0};
+  const float f1 = pow2(24), f2 = pow2(20);  // the units of the two kinds of rows
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -548,133 +672,123 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_split_kernel(co
       const int row = 8 * j + 2 * cq + c;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], off);
-      if (r == 0) {
-        s_m[warp][row] = m[j][c];
-        s_l[warp][row] = l[j][c];
-      }
+      const int rr = done.r0 + row;
+      const float inv = 1.f / l[j][c];  // no key: 0 / 0
 #pragma unroll
       for (int g = 0; g < W; ++g) {
         const float z = __shfl_sync(0xffffffffu, accz[j][c], 4 * g + cq);
-        *reinterpret_cast<float4 *>(mine + row * D + 32 * g + 4 * r) =
-            make_float4(fmaf(acc[g][0][j][c], f1, z), fmaf(acc[g][0][j][c + 2], f2, z),
-                        fmaf(acc[g][1][j][c], f1, z), fmaf(acc[g][1][j][c + 2], f2, z));
+        const float4 v = make_float4(fmaf(acc[g][0][j][c], f1, z), fmaf(acc[g][0][j][c + 2], f2, z),
+                                     fmaf(acc[g][1][j][c], f1, z), fmaf(acc[g][1][j][c + 2], f2, z));
+        if (row >= done.nr) continue;
+        if (whole) {
+          T *o = static_cast<T *>(a.o) + (done.row0 + rr / a.G) * a.so0 + (done_hk * a.G + rr % a.G) * a.so1;
+          *reinterpret_cast<uint2 *>(o + 32 * g + 4 * r) =
+              make_uint2(Pack2<T>::pack(v.x * inv, v.y * inv), Pack2<T>::pack(v.z * inv, v.w * inv));
+        } else {
+          *reinterpret_cast<float4 *>(a.ws_acc + (slot * ROWS + row) * D + 32 * g + 4 * r) = v;
+        }
       }
+      if (!whole && r == 0)  // (a sum that is no number counts)
+        a.ws_ml[slot * ROWS + row] = make_float2(l[j][c] == 0.f ? -INFINITY : mu[j][c], l[j][c]);
     }
-  __syncthreads();
-  const int64_t slot0 = ((static_cast<int64_t>(brt) * a.Hkv + hk) * a.splits + split) * ROWS;
-  for (int i = tid; i < pl.nr * (D / 8); i += kThreads) {
-    const int row = i / (D / 8), d = (i % (D / 8)) * 8;
-    float top = s_m[0][row];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][row]);
-    float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (s_m[w][row] == -INFINITY) continue;  // this warp has nothing for the row
-      const float f = ex2_approx(s_m[w][row] - top);
-      const float4 *p = reinterpret_cast<const float4 *>(smem + w * RING) + (row * D + d) / 4;
-      const float4 x = p[0], y = p[1];
-      sum = fmaf(s_l[w][row], f, sum);
-      v[0] = fmaf(x.x, f, v[0]); v[1] = fmaf(x.y, f, v[1]); v[2] = fmaf(x.z, f, v[2]); v[3] = fmaf(x.w, f, v[3]);
-      v[4] = fmaf(y.x, f, v[4]); v[5] = fmaf(y.y, f, v[5]); v[6] = fmaf(y.z, f, v[6]); v[7] = fmaf(y.w, f, v[7]);
-    }
-    if (a.splits == 1) {
-      const int rr = pl.r0 + row;
-      T *o = static_cast<T *>(a.o) + (pl.row0 + rr / a.G) * a.so0 + (hk * a.G + rr % a.G) * a.so1 + d;
-      uint4 out;
-      out.x = Pack2<T>::pack(v[0] / sum, v[1] / sum);
-      out.y = Pack2<T>::pack(v[2] / sum, v[3] / sum);
-      out.z = Pack2<T>::pack(v[4] / sum, v[5] / sum);
-      out.w = Pack2<T>::pack(v[6] / sum, v[7] / sum);
-      *reinterpret_cast<uint4 *>(o) = out;
-    } else {
-      float4 *p = reinterpret_cast<float4 *>(a.ws_acc + (slot0 + row) * D + d);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
-      if (d == 0) *reinterpret_cast<float2 *>(a.ws_ml + 2 * (slot0 + row)) = make_float2(top, sum);
-    }
+  if (!more) break;
+  at_start = false;
   }
 }
 
-// One warp per query row: adds up the splits that have keys for its row tile.
+// One CTA per worker: the row tile that starts in its last segment and goes on in later workers, if
+// any. Its first part is in that worker's slot, the others in the first slots of the workers after it.
+// A warp adds up a row; each lane weighs one of 32 parts, so the parts' loads do not wait for one
+// another, and 16 are in flight. Launched while the main kernel ends, it waits for it first.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * ROWS) kv4_merge_kernel(const Args a) {
   constexpr int E = D / 32;
-  const int64_t row_all = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int64_t tile = row_all / ROWS;
-  const int row = static_cast<int>(row_all % ROWS);
-  if (tile >= static_cast<int64_t>(a.B) * a.n_rt * a.Hkv) return;
-  const int hk = static_cast<int>(tile % a.Hkv), brt = static_cast<int>(tile / a.Hkv);
-  Place pl;
-  if (!locate<ROWS>(a, brt / a.n_rt, brt % a.n_rt, hk, pl) || row >= pl.nr) return;
-  const int used = max((pl.seen + a.chunk - 1) / a.chunk, 1);
-  const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + tile * a.splits * ROWS + row;
-  const float *acc = a.ws_acc + (tile * a.splits * ROWS + row) * D + lane * E;
-  float top = -INFINITY;
-  for (int s = lane; s < used; s += 32) top = fmaxf(top, ml[s * ROWS].x);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int worker = blockIdx.x, lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int4 *info = reinterpret_cast<const int4 *>(a.ws_open + worker);
+  const int4 o0 = info[0], o1 = info[1];
+  const Open open = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, 0, 0};
+  if (open.workers <= 1 || row >= open.nr) return;
+  auto at = [&](int i) { return (i == 0 ? static_cast<int64_t>(open.slot) : 2LL * (worker + i)) * ROWS + row; };
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < open.workers) ml = a.ws_ml[at(lane)];
+  float top = ml.x;
+  for (int i = lane + 32; i < open.workers; i += 32) top = fmaxf(top, a.ws_ml[at(i)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   float sum = 0.f, v[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < used; ++s) {
-    const float2 x = ml[s * ROWS];
-    const float f = x.x == -INFINITY ? 0.f : ex2_approx(x.x - top);
-    sum = fmaf(x.y, f, sum);
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = fmaf(acc[static_cast<int64_t>(s) * ROWS * D + i], f, v[i]);
+  for (int d = 0; d < E; ++d) v[d] = 0.f;
+  for (int i0 = 0; i0 < open.workers; i0 += 32) {
+    if (i0 > 0) ml = i0 + lane < open.workers ? a.ws_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    const int n = min(32, open.workers - i0);
+#pragma unroll 16
+    for (int i = 0; i < n; ++i) {
+      const float *acc = a.ws_acc + at(i0 + i) * D + lane * E;
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(acc);
+        v[0] = fmaf(x.x, fi, v[0]); v[1] = fmaf(x.y, fi, v[1]); v[2] = fmaf(x.z, fi, v[2]); v[3] = fmaf(x.w, fi, v[3]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2 *>(acc);
+        v[0] = fmaf(x.x, fi, v[0]); v[1] = fmaf(x.y, fi, v[1]);
+      }
+    }
   }
-  const int rr = pl.r0 + row;
-  T *o = static_cast<T *>(a.o) + (pl.row0 + rr / a.G) * a.so0 + (hk * a.G + rr % a.G) * a.so1 + lane * E;
 #pragma unroll
-  for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t *>(o + i) = Pack2<T>::pack(v[i] / sum, v[i + 1] / sum);
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  const int rr = open.r0 + row;
+  T *o = static_cast<T *>(a.o) + (open.row0 + rr / a.G) * a.so0 + (open.hk * a.G + rr % a.G) * a.so1 + lane * E;
+#pragma unroll
+  for (int d = 0; d < E; d += 2) *reinterpret_cast<uint32_t *>(o + d) = Pack2<T>::pack(v[d] / sum, v[d + 1] / sum);
 }
 
 struct Plan {
-  int nt = 1, n_rt = 1, splits = 1, chunk = 128;
-  size_t ml_bytes = 0, ws_bytes = 0;
+  int nt = 1, n_rt = 1, ctas = 0;
+  size_t ml_at = 0, acc_at = 0, ws_bytes = 0;
 };
 
-// Row tiles of 8 rows where all of a sequence's rows fit one, else of 16; key splits for four waves
-// of CTAs, in chunks between 128 tokens (a tile per warp) and 2048.
+// Row tiles of 8 rows where all of a sequence's rows fit one, else of 16; one wave of CTAs, fewer where
+// they would not all have tiles.
 Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t D, int64_t block_size,
                int64_t max_blocks) {
   Plan p;
   const int64_t rows = std::max<int64_t>(max_new, 1) * (Hq / Hkv);
   p.nt = rows <= 8 ? 1 : 2;
   p.n_rt = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
-  const int64_t tiles = B * p.n_rt * Hkv, most = max_blocks * block_size;
-  const int64_t want = 16LL * (sm_count() > 0 ? sm_count() : 148);
-  int64_t chunk = 2048;
-  while (chunk > 128 && tiles * ((most + chunk - 1) / chunk) < want) chunk /= 2;
-  p.chunk = static_cast<int>(chunk);
-  p.splits = static_cast<int>(std::max<int64_t>((most + chunk - 1) / chunk, 1));
-  if (p.splits > 1) {
-    const size_t slots = static_cast<size_t>(tiles) * p.splits * 8 * p.nt;
-    p.ml_bytes = (slots * 2 * sizeof(float) + 255) / 256 * 256;
-    p.ws_bytes = p.ml_bytes + slots * D * sizeof(float);
-  }
+  const int64_t most = B * p.n_rt * Hkv * std::max<int64_t>((max_blocks * block_size + kTile - 1) / kTile, 1);
+  const int64_t wave = (sm_count() > 0 ? sm_count() : 148) * 3;
+  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(wave, (most + kWarps * kMinTiles - 1) / (kWarps * kMinTiles))));
+  const size_t workers = static_cast<size_t>(p.ctas) * kWarps, rows_all = 2 * workers * 8 * p.nt;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  p.ml_at = up(workers * sizeof(Open));
+  p.acc_at = up(p.ml_at + rows_all * sizeof(float2));
+  p.ws_bytes = p.acc_at + rows_all * D * sizeof(float);
   return p;
 }
 
 template <typename T, int D, int NT>
 int launch(const Args &a, cudaStream_t st) {
   auto kern = kv4_split_kernel<T, D, NT>;
-  constexpr int smem = kWarps * kStages * 2 * Piece<D>::BYTES;
+  constexpr int smem = kWarps * (kStages * 2 * Piece<D>::BYTES + NT * Piece<D>::W * 512);
   KernelLaunchInfo info;
   const int rc = prepare_kernel(reinterpret_cast<const void *>(kern), smem, kThreads, 1, &info);
   if (rc) return rc;
-  const int64_t tiles = static_cast<int64_t>(a.B) * a.n_rt * a.Hkv;
-  kern<<<static_cast<unsigned>(tiles * a.splits + 1), kThreads, smem, st>>>(a);
+  kern<<<a.workers / kWarps, kThreads, smem, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_status(e, "paged kv4 attention launch");
-  if (a.splits > 1 && tiles > 0) {
-    const unsigned grid = static_cast<unsigned>((tiles * 8 * NT + kWarps - 1) / kWarps);
-    kv4_merge_kernel<T, D, 8 * NT><<<grid, kThreads, 0, st>>>(a);
-    e = cudaGetLastError();
-  }
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.workers);
+  cfg.blockDim = dim3(32 * 8 * NT);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kv4_merge_kernel<T, D, 8 * NT>, a);
   return cuda_status(e, "paged kv4 attention merge launch");
 }
 
@@ -693,9 +807,9 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" size_t tllm_paged_kv4_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
                                                      int64_t max_new, int64_t D, int64_t block_size,
                                                      int64_t max_blocks) {
-  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_new < 0 || D <= 0 || block_size <= 0 || max_blocks <= 0)
+  if (B < 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_new < 0 || D <= 0 || block_size <= 0 || max_blocks < 0)
     return 0;
-  return tllm::kv4::make_plan(B, Hq, Hkv, max_new, D, block_size, max_blocks).ws_bytes;
+  return tllm::kv4::make_plan(B, Hq, Hkv, std::min(max_new, T), D, block_size, max_blocks).ws_bytes;
 }
 
 extern "C" int tllm_paged_kv4_attn(const void *q, const void *cache, const int32_t *block_tables,
@@ -756,19 +870,18 @@ extern "C" int tllm_paged_kv4_attn(const void *q, const void *cache, const int32
   a.scale_log2 = sm_scale * kLog2e;
   a.max_new = static_cast<int>(std::min<int64_t>(max_new, T));
   const Plan pl = make_plan(B, Hq, Hkv, a.max_new, D, block_size, max_blocks);
-  TLLM_CHECK_ARG(B * pl.n_rt * Hkv * pl.splits < (1LL << 31) - 1, "paged_kv4_attn: grid too large");
+  TLLM_CHECK_ARG(static_cast<int64_t>(pl.n_rt) * Hkv < (1LL << 31), "paged_kv4_attn: problem too large");
   a.n_rt = pl.n_rt;
-  a.splits = pl.splits;
-  a.chunk = pl.chunk;
-  if (pl.ws_bytes > 0) {
-    if (!workspace || workspace_bytes < pl.ws_bytes)
-      return fail(TLLM_ERR_WORKSPACE, "paged_kv4_attn: workspace of %zu bytes needed, %zu given", pl.ws_bytes,
-                  workspace_bytes);
-    TLLM_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
-                   "paged_kv4_attn: workspace must be 256-byte aligned");
-    a.ws_ml = static_cast<float *>(workspace);
-    a.ws_acc = reinterpret_cast<float *>(static_cast<char *>(workspace) + pl.ml_bytes);
-  }
+  a.workers = pl.ctas * kWarps;
+  if (!workspace || workspace_bytes < pl.ws_bytes)
+    return fail(TLLM_ERR_WORKSPACE, "paged_kv4_attn: workspace of %zu bytes needed, %zu given", pl.ws_bytes,
+                workspace_bytes);
+  TLLM_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+                 "paged_kv4_attn: workspace must be 256-byte aligned");
+  char *ws = static_cast<char *>(workspace);
+  a.ws_open = reinterpret_cast<Open *>(ws);
+  a.ws_ml = reinterpret_cast<float2 *>(ws + pl.ml_at);
+  a.ws_acc = reinterpret_cast<float *>(ws + pl.acc_at);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == TLLM_DTYPE_F16 ? launch_d<__half>(a, D, pl.nt, st) : launch_d<__nv_bfloat16>(a, D, pl.nt, st);
 }
