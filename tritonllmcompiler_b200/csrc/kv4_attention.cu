@@ -37,6 +37,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 32;   // tokens a warp takes at a time: two pieces
 constexpr int kStages = 2;  // tiles of a warp in shared memory
+constexpr int kMergeLoads = 8;  // parts a merging warp reads at a time
 constexpr int kMinTiles = 2;  // a warp's least run of tiles
 
 enum : int { SITE_TILE = 0x41 };
@@ -146,7 +147,7 @@ __device__ __forceinline__ uint32_t pick(const uint32_t (&v)[W], int r) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
 template <int N>
-__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
   static_assert(N == 1 || N == 2 || N == 4, "vector width");
   if constexpr (N == 4) {
     const uint4 v = *reinterpret_cast<const uint4 *>(p);
@@ -447,10 +448,10 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint8_t *pb = base + h * P::BYTES;
-      lds_words<W>(pb + P::K_CODES + r * (D / 2) + cq * (4 * W), k0[h]);
-      lds_words<W>(pb + P::K_CODES + (r + 8) * (D / 2) + cq * (4 * W), k1[h]);
-      lds_words<W / 2>(pb + P::k_scale(r, 0), s0[h]);
-      lds_words<W / 2>(pb + P::k_scale(r + 8, 0), s1[h]);
+      load_words<W>(pb + P::K_CODES + r * (D / 2) + cq * (4 * W), k0[h]);
+      load_words<W>(pb + P::K_CODES + (r + 8) * (D / 2) + cq * (4 * W), k1[h]);
+      load_words<W / 2>(pb + P::k_scale(r, 0), s0[h]);
+      load_words<W / 2>(pb + P::k_scale(r + 8, 0), s1[h]);
       uint32_t z0 = 0, z1 = 0;
       if (W == 4 || cq < 2) {
         const uint8_t *zp = pb + P::k_zero(r, 0) + 4 * (cq % (W / 2));
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
     int e;  // exponent field of the tile's largest V scale
     {
       uint32_t v[W / 2], big = 0;
-      lds_words<W / 2>(base + (lane >> 4) * P::BYTES + P::V_SCALE + (lane & 15) * 2 * W, v);
+      load_words<W / 2>(base + (lane >> 4) * P::BYTES + P::V_SCALE + (lane & 15) * 2 * W, v);
 #pragma unroll
       for (int i = 0; i < W / 2; ++i) big = __vmaxu2(big, v[i] & 0x7fff7fffu);
       e = static_cast<int>(__reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16)) >> 10);
@@ -553,10 +554,10 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       const uint8_t *pb = base + h * P::BYTES;
       // Token pairs cq and cq + 4: scales of both tokens per group, zeros of group r % W, codes.
       uint32_t sw[W], s0[W], s1[W];
-      lds_words<W>(pb + P::v_scale(2 * cq, 0), sw);
+      load_words<W>(pb + P::v_scale(2 * cq, 0), sw);
 #pragma unroll
       for (int g = 0; g < W; ++g) s0[g] = __byte_perm(sw[g / 2], sw[W / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410);
-      lds_words<W>(pb + P::v_scale(2 * cq + 8, 0), sw);
+      load_words<W>(pb + P::v_scale(2 * cq + 8, 0), sw);
 #pragma unroll
       for (int g = 0; g < W; ++g) s1[g] = __byte_perm(sw[g / 2], sw[W / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410);
       const uint8_t *zp = pb + P::v_zero(2 * cq, r % W);
@@ -569,8 +570,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       }
       const uint8_t *vp = pb + P::V_CODES + cq * D + (r ^ P::swizzle(cq)) * P::CHUNK;
       uint32_t v0[W], v1[W];
-      lds_words<W>(vp, v0);
-      lds_words<W>(vp + 4 * D, v1);
+      load_words<W>(vp, v0);
+      load_words<W>(vp + 4 * D, v1);
       uint32_t b0[NT], b1[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -699,9 +700,9 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
 // One CTA per worker: the row tile that starts in its last segment and goes on in later workers, if
 // any. Its first part is in that worker's slot, the others in the first slots of the workers after it.
 // A warp adds up a row; each lane weighs one of 32 parts, so the parts' loads do not wait for one
-// another, and 16 are in flight. Launched while the main kernel ends, it waits for it first.
+// another, and 8 are in flight. Launched while the main kernel ends, it waits for it first.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(32 * ROWS) kv4_merge_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * ROWS, 1) kv4_merge_kernel(const Args a) {
   constexpr int E = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int worker = blockIdx.x, lane = threadIdx.x & 31, row = threadIdx.x >> 5;
@@ -724,16 +725,23 @@ __global__ void __launch_bounds__(32 * ROWS) kv4_merge_kernel(const Args a) {
     const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
     sum = fmaf(ml.y, f, sum);
     const int n = min(32, open.workers - i0);
-#pragma unroll 16
-    for (int i = 0; i < n; ++i) {
-      const float *acc = a.ws_acc + at(i0 + i) * D + lane * E;
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if constexpr (E == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(acc);
-        v[0] = fmaf(x.x, fi, v[0]); v[1] = fmaf(x.y, fi, v[1]); v[2] = fmaf(x.z, fi, v[2]); v[3] = fmaf(x.w, fi, v[3]);
-      } else {
-        const float2 x = *reinterpret_cast<const float2 *>(acc);
-        v[0] = fmaf(x.x, fi, v[0]); v[1] = fmaf(x.y, fi, v[1]);
+    for (int i1 = 0; i1 < n; i1 += kMergeLoads) {
+      uint32_t x[kMergeLoads][E];
+#pragma unroll
+      for (int i = 0; i < kMergeLoads; ++i) {
+        if (i1 + i < n) {
+          const uint8_t *acc = reinterpret_cast<const uint8_t *>(a.ws_acc + at(i0 + i1 + i) * D + lane * E);
+          load_words<E>(acc, x[i]);
+        } else {
+#pragma unroll
+          for (int d = 0; d < E; ++d) x[i][d] = 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kMergeLoads; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);  // (0 past the last part)
+#pragma unroll
+        for (int d = 0; d < E; ++d) v[d] = fmaf(__uint_as_float(x[i][d]), fi, v[d]);
       }
     }
   }
