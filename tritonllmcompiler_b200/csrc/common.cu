@@ -211,6 +211,7 @@ int qkv_read_status(int *out);
 int qknr_read_status(int *out);
 int kv4_read_status(int *out);
 int kv4a_read_status(int *out);
+int kv4p_read_status(int *out);
 namespace paged {
 int read_status(int *out);
 }
@@ -219,7 +220,8 @@ int read_and_clear_device_status(int *out) {
   int (*readers[])(int *) = {flash_read_status, swiglu_read_status, paged::read_status,
                              selftest_read_status, pkv_read_status, ppf_read_status,
                              fbwd_read_status, swiglu8_read_status, qkv_read_status,
-                             qknr_read_status, kv4_read_status, kv4a_read_status};
+                             qknr_read_status, kv4_read_status, kv4a_read_status,
+                             kv4p_read_status};
   int first = 0;
   for (auto rd : readers) {
     int v = 0;

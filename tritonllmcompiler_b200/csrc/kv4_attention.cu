@@ -10,9 +10,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.h"
-#include "kv4.cuh"
-#include "ptx.cuh"
+#include "kv4_attention.cuh"
 
 namespace tllm {
 
@@ -32,70 +30,15 @@ int kv4a_read_status(int *out) {
 namespace kv4 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 32;   // tokens a warp takes at a time: two pieces
 constexpr int kStages = 2;  // tiles of a warp in shared memory
 constexpr int kMergeLoads = 8;  // parts a merging warp reads at a time
 constexpr int kMinTiles = 2;  // a warp's least run of tiles
+constexpr int kSplitRows = 32;  // query rows per sequence and KV head up to which kv4_split_kernel runs
 
 enum : int { SITE_TILE = 0x41 };
-
-// A row tile of several workers: rows [r0, r0 + nr) of the sequence that starts at row0.
-struct __align__(16) Open {
-  int workers, slot, hk, row0;  // workers 0: none; the first part's slot
-  int r0, nr, pad0, pad1;
-};
-
-struct Args {
-  const void *q;
-  const uint8_t *cache;
-  const int32_t *block_tables, *lens, *cu;
-  void *o;
-  // Partial results: two slots per worker (its first segment, its last), and per worker the row tile
-  // that starts in its last segment and goes on in the next workers.
-  Open *ws_open;    // [workers]
-  float2 *ws_ml;    // [slots][rows of a tile]: reference in log2 units, sum
-  float *ws_acc;    // [slots][rows of a tile][D]
-  int64_t sq0, sq1, so0, so1, sblk, shead, sbt0, sbt1;
-  int64_t T, num_blocks, max_blocks;
-  int B, Hkv, G, log2_bs, causal, max_new;
-  int n_rt, workers;  // row tiles per sequence and KV head; warps that share the tiles
-  float scale_log2;
-};
-
-// A row tile: rows r0 .. r0 + nr of the n_q * G rows of sequence b and a KV head hk, row r being new
-// token r / G of query head hk * G + r % G, and how many keys they see.
-struct Place {
-  int b, rt, r0, nr, row0, n_q, len, seen;
-};
-
-__device__ __forceinline__ int row_keys(const Args &a, const Place &p, int r) {
-  return a.causal ? min(max(p.len - p.n_q + r / a.G + 1, 0), p.len) : p.len;
-}
-
-template <int ROWS>
-__device__ __forceinline__ bool locate(const Args &a, int b, int rt, Place &p) {
-  p.b = b;
-  p.rt = rt;
-  const int lim = static_cast<int>(a.T);
-  p.row0 = min(max(__ldg(a.cu + b), 0), lim);
-  p.n_q = min(max(__ldg(a.cu + b + 1), p.row0), lim) - p.row0;
-  p.r0 = rt * ROWS;
-  p.nr = min(ROWS, p.n_q * a.G - p.r0);
-  if (p.nr <= 0) return false;
-  p.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.lens + b), 0)), a.max_blocks << a.log2_bs));
-  p.seen = row_keys(a, p, p.r0 + p.nr - 1);
-  return true;
-}
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -112,28 +55,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t pack_half(float a, float b) { return Pack2<__half>::pack(a, b); }
-
-__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 // All ones in the halves of v that are +0 (as the weights of hidden tokens are).
 __device__ __forceinline__ uint32_t zero_halves(uint32_t v) { return __vcmpeq2(v, 0u); }
 
@@ -142,22 +63,6 @@ template <int W>
 __device__ __forceinline__ uint32_t pick(const uint32_t (&v)[W], int r) {
   if constexpr (W == 2) return (r & 1) ? v[1] : v[0];
   else return (r & 2) ? ((r & 1) ? v[3] : v[2]) : ((r & 1) ? v[1] : v[0]);
-}
-
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
-
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
-  static_assert(N == 1 || N == 2 || N == 4, "vector width");
-  if constexpr (N == 4) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t *>(p);
-  }
 }
 
 // Four fp16 pairs from a word of two times four codes: x[0], x[2] are the codes of bits 0-3 and 8-11 of
@@ -171,19 +76,14 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
   x[2] = sub_half2(w, x[3]);  // exact, and not on the logic pipe, which is the busier one
 }
 
-// Key tiles of a row tile; one where its rows see nothing, so that somebody writes them.
-__device__ __forceinline__ int key_tiles(const Place &p) { return max((p.seen + kTile - 1) / kTile, 1); }
-
 // Few query rows per KV head (decode, speculative tokens): ROWS = 8 * NT rows a row tile.
 //
-// All key tiles of all row tiles form one line: sequences, in them row tiles, in them KV heads, in
-// them tiles of 32 keys. Every warp of the grid, one wave of CTAs, takes an equal run of it (within a
-// tile), whatever the lengths are; each CTA finds its place by a scan over the sequences. A warp
-// works by itself: its own ring of bulk copies (a page's K and V of one head are contiguous), its
-// own running maximum and sum. A row tile that lies whole in a run is stored at once; otherwise each warp
-// stores its part, and kv4_merge_kernel adds the parts up. (CTAs of one row tile and 1024 keys
-// each, as before, spent 5 us of latency per CTA in starting and joining: 115 against @A us for 64
-// requests of U[512, 8192], 32 heads over 8.)
+// A worker of the line (kv4_attention.cuh) is a warp, and the grid one wave of CTAs. A warp works by
+// itself: its own ring of bulk copies (a page's K and V of one head are contiguous), its own running
+// maximum and sum. A row tile that lies whole in a run is stored at once; otherwise each warp stores
+// its part, and kv4_merge_kernel adds the parts up. (CTAs of one row tile and 1024 keys each, as
+// before, spent 5 us of latency per CTA in starting and joining: 115 against 101 us for 64 requests of
+// U[512, 8192], 32 heads over 8.)
 //
 // Both products run as 16 x 8 x 16 MMAs with the cache as the 16-row operand, so 8 query rows fill
 // them: S^T = K Q^T and O^T = V^T P^T. The operands from the cache are the codes themselves, as fp16
@@ -210,8 +110,8 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
   constexpr int TILE_BYTES = 2 * P::BYTES;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[kWarps][kStages];
-  __shared__ int64_t s_scan[kWarps], s_off[kWarps];
-  __shared__ int s_seq[kWarps], s_abort;
+  __shared__ LineScan<kThreads, kWarps> s_line;
+  __shared__ int s_abort;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, cq = lane & 3;  // fragment row (token, channel or query row) and column pair
@@ -221,85 +121,16 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
     s_abort = 0;
     fence_mbar_init();
   }
-
-  // ---- the line and this warp's run of it ----
+  int64_t per, total;
+  scan_line<ROWS, kTile>(a, s_line, kMinTiles, per, total, &g_kv4a_status);
+  clear_rows<T, D>(a);
   const int worker = blockIdx.x * kWarps + warp;
-  const int share = (a.B + kThreads - 1) / kThreads;
-  const int b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
-  auto tiles_of_seq = [&](int b) {
-    int64_t t = 0;
-    Place p;
-    for (int rt = 0; rt < a.n_rt && locate<ROWS>(a, b, rt, p); ++rt) t += key_tiles(p);
-    if (p.n_q > a.max_new) atomicCAS(&g_kv4a_status, 0, TLLM_DEV_BAD_INDEX);
-    return t * a.Hkv;
-  };
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of_seq(b);
-  int64_t upto = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += u;
-  }
-  if (lane == 31) s_scan[warp] = upto;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += s_scan[w];
-    total += s_scan[w];
-  }
-  const int64_t per = max((total + a.workers - 1) / a.workers, static_cast<int64_t>(kMinTiles));
-  for (int w = 0; w < kWarps; ++w) {
-    int64_t off = (static_cast<int64_t>(blockIdx.x) * kWarps + w) * per - (upto - mine);
-    if (off < 0 || off >= mine) continue;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t t = tiles_of_seq(b);
-      if (off < t) {
-        s_seq[w] = b;
-        s_off[w] = off;
-        break;
-      }
-      off -= t;
-    }
-  }
-  // Rows that belong to no sequence are cleared.
-  {
-    const int64_t from = a.B > 0 ? min(max(static_cast<int64_t>(__ldg(a.cu + a.B)), int64_t{0}), a.T) : 0;
-    const int hq = a.Hkv * a.G;
-    const int64_t n = (a.T - from) * hq * (D / 8);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < n; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-      const int64_t row = i / (D / 8);
-      T *o = static_cast<T *>(a.o) + (from + row / hq) * a.so0 + (row % hq) * a.so1;
-      *reinterpret_cast<uint4 *>(o + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-    }
-  }
-  __syncthreads();
   if (lane == 0) a.ws_open[worker].workers = 0;
   int64_t pos = worker * per;
   const int64_t end = min(pos + per, total);
-  if (pos >= end) return;
-  Place pl;
-  int nt, hk, first;  // the segment's row tile has nt key tiles; the segment starts at `first`
-  {
-    int64_t off = s_off[warp];
-    int b = s_seq[warp], rt = 0;
-    while (b < a.B) {  // (always found: pos < total)
-      if (locate<ROWS>(a, b, rt, pl)) {
-        nt = key_tiles(pl);
-        if (off < static_cast<int64_t>(nt) * a.Hkv) break;
-        off -= static_cast<int64_t>(nt) * a.Hkv;
-      }
-      if (++rt == a.n_rt) {
-        rt = 0;
-        ++b;
-      }
-    }
-    if (b == a.B) return;
-    hk = static_cast<int>(off / nt);
-    first = static_cast<int>(off % nt);
-  }
-  int count = static_cast<int>(min(static_cast<int64_t>(nt - first), end - pos));
+  Segment sg;
+  if (pos >= end || !first_segment<ROWS, kTile>(a, s_line.seq[warp], s_line.off[warp], end - pos, sg)) return;
+  const Place &pl = sg.pl;
   bool at_start = true;  // the worker's first segment
 
   // ---- the warp's ring ----
@@ -311,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
   // Starts the copy of the segment's tile k, `ahead` tiles after the next one to be taken.
   auto issue = [&](int k, int ahead) {
     if ((k & 31) == 0) {
-      const int tok = (first + k + lane) * kTile;
+      const int tok = (sg.first + k + lane) * kTile;
       auto page = [&](int t) -> int {
         if (t >= pl.seen) return 0;
         const int p = __ldg(a.block_tables + pl.b * a.sbt0 + (t >> a.log2_bs) * a.sbt1);
@@ -319,21 +150,21 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
         atomicCAS(&g_kv4a_status, 0, TLLM_DEV_BAD_INDEX);
         return 0;
       };
-      if (k + lane < count) {
+      if (k + lane < sg.count) {
         page0 = page(tok);
         if (a.log2_bs == 4) page1 = page(tok + kPieceTokens);
       }
     }
     if (lane == (k & 31)) {  // the lane that has the pages
-      const int tok = (first + k) * kTile;
+      const int tok = (sg.first + k) * kTile;
       const bool both = pl.seen - tok > kPieceTokens;
       const uint32_t stage = (taken + ahead) % kStages;
       const uint32_t bar = smem_u32(&s_bar[warp][stage]), dst = smem_u32(ring) + stage * TILE_BYTES;
-      const uint8_t *src = a.cache + hk * a.shead + page0 * a.sblk;
+      const uint8_t *src = a.cache + sg.hk * a.shead + page0 * a.sblk;
       mbar_arrive_expect_tx(bar, both ? TILE_BYTES : P::BYTES);
       if (a.log2_bs == 4) {
         bulk_load(dst, src, P::BYTES, bar);
-        if (both) bulk_load(dst + P::BYTES, a.cache + hk * a.shead + page1 * a.sblk, P::BYTES, bar);
+        if (both) bulk_load(dst + P::BYTES, a.cache + sg.hk * a.shead + page1 * a.sblk, P::BYTES, bar);
       } else {
         const int piece = (tok & ((1 << a.log2_bs) - 1)) / kPieceTokens;
         bulk_load(dst, src + piece * P::BYTES, both ? TILE_BYTES : P::BYTES, bar);
@@ -341,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
     }
   };
   auto prime = [&] {
-    for (int k = 0; k < kStages && k < count && pl.seen > 0; ++k) issue(k, k);
+    for (int k = 0; k < kStages && k < sg.count && pl.seen > 0; ++k) issue(k, k);
   };
   prime();
 
@@ -360,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       uint4 raw = make_uint4(0, 0, 0, 0);
       if (ok)
         raw = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (pl.row0 + row / a.G) * a.sq0 +
-                                                    (hk * a.G + row % a.G) * a.sq1 + 32 * w + 8 * cq));
+                                                    (sg.hk * a.G + row % a.G) * a.sq1 + 32 * w + 8 * cq));
       const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -611,13 +442,13 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
   };
 
   bool ok = true;
-  for (int k = 0; k < count && pl.seen > 0; ++k, ++taken) {
+  for (int k = 0; k < sg.count && pl.seen > 0; ++k, ++taken) {
     const uint32_t stage = taken % kStages, bar = smem_u32(&s_bar[warp][stage]), parity = (taken / kStages) & 1;
     if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
       ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &s_abort, &g_kv4a_status, TLLM_DEV_WAIT_TIMEOUT + SITE_TILE));
     if (!ok) {
       // The copies in flight still write to this CTA's memory: give them their time, then leave.
-      for (int i = 0; i < kStages && k + i < count; ++i) {
+      for (int i = 0; i < kStages && k + i < sg.count; ++i) {
         const long long since = clock64();
         while (!mbar_try_wait(smem_u32(&s_bar[warp][(taken + i) % kStages]), ((taken + i) / kStages) & 1) &&
                clock64() - since < kWaitLimitCycles) {
@@ -625,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       }
       return;
     }
-    const int at = (first + k) * kTile;
+    const int at = (sg.first + k) * kTile;
     uint8_t *base = ring + stage * TILE_BYTES;
     if (at + kTile > lim_all) {
       tile(base, at, std::true_type{});
@@ -634,37 +465,20 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       tile(base, at, std::false_type{});
     }
     __syncwarp();
-    if (k + kStages < count) issue(k + kStages, kStages);
+    if (k + kStages < sg.count) issue(k + kStages, kStages);
   }
 
   // ---- this segment's results; the next one's copies go out first ----
-  const Place done = pl;
-  const int done_hk = hk, done_first = first, done_count = count, done_nt = nt;
+  const Segment done = sg;
   const int64_t done_pos = pos;
-  pos += count;
-  const bool more = pos < end;
-  if (more) {
-    first = 0;
-    if (++hk == a.Hkv) {
-      hk = 0;
-      int b = pl.b, rt = pl.rt;
-      do {
-        if (++rt == a.n_rt) {
-          rt = 0;
-          ++b;
-        }
-      } while (b < a.B && !locate<ROWS>(a, b, rt, pl));
-      if (b == a.B) return;  // (always found: pos < total)
-      nt = key_tiles(pl);
-    }
-    count = static_cast<int>(min(static_cast<int64_t>(nt), end - pos));
-    prime();
-  }
-  const bool whole = done_count == done_nt;
+  pos += sg.count;
+  const bool more = next_segment<ROWS, kTile>(a, end - pos, sg);
+  if (more) prime();
+  const bool whole = done.count == done.nt;
   const int64_t slot = 2 * static_cast<int64_t>(worker) + (at_start ? 0 : 1);
-  if (!whole && done_first == 0 && lane == 0)
-    a.ws_open[worker] = Open{static_cast<int>((done_pos + done_nt - 1) / per) - worker + 1, static_cast<int>(slot),
-                             done_hk, done.row0, done.r0, done.nr, 0, 0};
+  if (!whole && done.first == 0 && lane == 0)
+    a.ws_open[worker] = Open{static_cast<int>((done_pos + done.nt - 1) / per) - worker + 1, static_cast<int>(slot),
+                             done.hk, done.pl.row0, done.pl.r0, done.pl.nr, 0, 0};
   const float f1 = pow2(24), f2 = pow2(20);  // the units of the two kinds of rows
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -673,16 +487,16 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
       const int row = 8 * j + 2 * cq + c;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], off);
-      const int rr = done.r0 + row;
+      const int rr = done.pl.r0 + row;
       const float inv = 1.f / l[j][c];  // no key: 0 / 0
 #pragma unroll
       for (int g = 0; g < W; ++g) {
         const float z = __shfl_sync(0xffffffffu, accz[j][c], 4 * g + cq);
         const float4 v = make_float4(fmaf(acc[g][0][j][c], f1, z), fmaf(acc[g][0][j][c + 2], f2, z),
                                      fmaf(acc[g][1][j][c], f1, z), fmaf(acc[g][1][j][c + 2], f2, z));
-        if (row >= done.nr) continue;
+        if (row >= done.pl.nr) continue;
         if (whole) {
-          T *o = static_cast<T *>(a.o) + (done.row0 + rr / a.G) * a.so0 + (done_hk * a.G + rr % a.G) * a.so1;
+          T *o = static_cast<T *>(a.o) + (done.pl.row0 + rr / a.G) * a.so0 + (done.hk * a.G + rr % a.G) * a.so1;
           *reinterpret_cast<uint2 *>(o + 32 * g + 4 * r) =
               make_uint2(Pack2<T>::pack(v.x * inv, v.y * inv), Pack2<T>::pack(v.z * inv, v.w * inv));
         } else {
@@ -697,15 +511,15 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
   }
 }
 
-// One CTA per worker: the row tile that starts in its last segment and goes on in later workers, if
+// A CTA per worker and 8 rows: the row tile that starts in its last segment and goes on in later workers, if
 // any. Its first part is in that worker's slot, the others in the first slots of the workers after it.
 // A warp adds up a row; each lane weighs one of 32 parts, so the parts' loads do not wait for one
 // another, and 8 are in flight. Launched while the main kernel ends, it waits for it first.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(32 * ROWS, 1) kv4_merge_kernel(const Args a) {
+__global__ void __launch_bounds__(256, 1) kv4_merge_kernel(const Args a) {
   constexpr int E = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int worker = blockIdx.x, lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int worker = blockIdx.x, lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int4 *info = reinterpret_cast<const int4 *>(a.ws_open + worker);
   const int4 o0 = info[0], o1 = info[1];
   const Open open = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, 0, 0};
@@ -754,22 +568,26 @@ __global__ void __launch_bounds__(32 * ROWS, 1) kv4_merge_kernel(const Args a) {
 }
 
 struct Plan {
-  int nt = 1, n_rt = 1, ctas = 0;
+  int nt = 1, n_rt = 1, ctas = 0;  // nt: 8-row tiles of a row tile, 0 for the prefill kernel
+  int workers = 0;
   size_t ml_at = 0, acc_at = 0, ws_bytes = 0;
 };
 
-// Row tiles of 8 rows where all of a sequence's rows fit one, else of 16; one wave of CTAs, fewer where
-// they would not all have tiles.
+// Row tiles of 8 rows where all of a sequence's rows fit one, else of 16, and the prefill kernel above
+// kSplitRows rows; one wave of CTAs, fewer where they would not all have tiles.
 Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t D, int64_t block_size,
                int64_t max_blocks) {
   Plan p;
   const int64_t rows = std::max<int64_t>(max_new, 1) * (Hq / Hkv);
-  p.nt = rows <= 8 ? 1 : 2;
-  p.n_rt = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
-  const int64_t most = B * p.n_rt * Hkv * std::max<int64_t>((max_blocks * block_size + kTile - 1) / kTile, 1);
-  const int64_t wave = (sm_count() > 0 ? sm_count() : 148) * 3;
-  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(wave, (most + kWarps * kMinTiles - 1) / (kWarps * kMinTiles))));
-  const size_t workers = static_cast<size_t>(p.ctas) * kWarps, rows_all = 2 * workers * 8 * p.nt;
+  p.nt = rows <= 8 ? 1 : (rows <= kSplitRows ? 2 : 0);
+  const int row_tile = p.nt > 0 ? 8 * p.nt : kPrefillRows, tile = p.nt > 0 ? kTile : 128;
+  p.n_rt = static_cast<int>((rows + row_tile - 1) / row_tile);
+  const int64_t sms = sm_count() > 0 ? sm_count() : 148;
+  const int64_t most = B * p.n_rt * Hkv * std::max<int64_t>((max_blocks * block_size + tile - 1) / tile, 1);
+  const int64_t each = p.nt > 0 ? kWarps * kMinTiles : 1;  // a CTA's least run
+  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(p.nt > 0 ? 3 * sms : sms, (most + each - 1) / each)));
+  p.workers = p.ctas * (p.nt > 0 ? kWarps : 1);
+  const size_t workers = static_cast<size_t>(p.workers), rows_all = 2 * workers * row_tile;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   p.ml_at = up(workers * sizeof(Open));
   p.acc_at = up(p.ml_at + rows_all * sizeof(float2));
@@ -777,33 +595,43 @@ Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t D, i
   return p;
 }
 
+template <typename T, int D, int ROWS>
+int launch_merge(const Args &a, cudaStream_t st) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.workers, ROWS / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<T, D, ROWS>, a), "paged kv4 attention merge launch");
+}
+
 template <typename T, int D, int NT>
 int launch(const Args &a, cudaStream_t st) {
   auto kern = kv4_split_kernel<T, D, NT>;
   constexpr int smem = kWarps * (kStages * 2 * Piece<D>::BYTES + NT * Piece<D>::W * 512);
   KernelLaunchInfo info;
-  const int rc = prepare_kernel(reinterpret_cast<const void *>(kern), smem, kThreads, 1, &info);
+  int rc = prepare_kernel(reinterpret_cast<const void *>(kern), smem, kThreads, 1, &info);
   if (rc) return rc;
   kern<<<a.workers / kWarps, kThreads, smem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_status(e, "paged kv4 attention launch");
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.workers);
-  cfg.blockDim = dim3(32 * 8 * NT);
-  cfg.stream = st;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv4_merge_kernel<T, D, 8 * NT>, a);
-  return cuda_status(e, "paged kv4 attention merge launch");
+  rc = cuda_status(cudaGetLastError(), "paged kv4 attention launch");
+  return rc ? rc : launch_merge<T, D, 8 * NT>(a, st);
+}
+
+template <typename T, int D>
+int launch_nt(const Args &a, int nt, int dtype, cudaStream_t st) {
+  if (nt == 1) return launch<T, D, 1>(a, st);
+  if (nt == 2) return launch<T, D, 2>(a, st);
+  const int rc = launch_prefill(a, D, dtype, st);
+  return rc ? rc : launch_merge<T, D, kPrefillRows>(a, st);
 }
 
 template <typename T>
-int launch_d(const Args &a, int64_t D, int nt, cudaStream_t st) {
-  if (D == 64) return nt == 1 ? launch<T, 64, 1>(a, st) : launch<T, 64, 2>(a, st);
-  return nt == 1 ? launch<T, 128, 1>(a, st) : launch<T, 128, 2>(a, st);
+int launch_d(const Args &a, int64_t D, int nt, int dtype, cudaStream_t st) {
+  return D == 64 ? launch_nt<T, 64>(a, nt, dtype, st) : launch_nt<T, 128>(a, nt, dtype, st);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -880,7 +708,7 @@ extern "C" int tllm_paged_kv4_attn(const void *q, const void *cache, const int32
   const Plan pl = make_plan(B, Hq, Hkv, a.max_new, D, block_size, max_blocks);
   TLLM_CHECK_ARG(static_cast<int64_t>(pl.n_rt) * Hkv < (1LL << 31), "paged_kv4_attn: problem too large");
   a.n_rt = pl.n_rt;
-  a.workers = pl.ctas * kWarps;
+  a.workers = pl.workers;
   if (!workspace || workspace_bytes < pl.ws_bytes)
     return fail(TLLM_ERR_WORKSPACE, "paged_kv4_attn: workspace of %zu bytes needed, %zu given", pl.ws_bytes,
                 workspace_bytes);
@@ -891,5 +719,5 @@ extern "C" int tllm_paged_kv4_attn(const void *q, const void *cache, const int32
   a.ws_ml = reinterpret_cast<float2 *>(ws + pl.ml_at);
   a.ws_acc = reinterpret_cast<float *>(ws + pl.acc_at);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == TLLM_DTYPE_F16 ? launch_d<__half>(a, D, pl.nt, st) : launch_d<__nv_bfloat16>(a, D, pl.nt, st);
+  return dtype == TLLM_DTYPE_F16 ? launch_d<__half>(a, D, pl.nt, dtype, st) : launch_d<__nv_bfloat16>(a, D, pl.nt, dtype, st);
 }

@@ -1,0 +1,606 @@
+// Attention over the 4-bit paged cache for many query rows per KV head (prefill chunks): tcgen05 on
+// tiles of 128 query rows and 128 keys, the keys and values brought to fp16 on the way.
+//
+// A worker of the line (kv4_attention.cuh) is a CTA, one per SM; row tiles have 128 rows, key tiles
+// 128 keys. Work goes through rings of two stages:
+//   warp 5        copies: the tile's pages, K and V of one head, by bulk copies into the raw ring
+//   warps 8-15    unpack, a piece of 16 tokens each: code * scale + zero in fp16 (11 bits: an error of
+//                 2^-12 of a value against the half step of 1/30 of its group's range that 4 bits
+//                 cost), stored swizzled as the K and V operands
+//   warp 4        TMEM allocation and the lane that issues the UMMAs: S = Q K^T into one of two TMEM
+//                 buffers (the next tile's overlaps this tile's softmax), O += P V with P from TMEM
+//   warps 0-3     one query row per thread: q to fp16 (bf16 rows by a power of two that keeps them in
+//                 its range), softmax with a lazy rescale of O (2^8), the results
+// V's columns are stored in the order 0 4 1 5 2 6 3 7 of every eight channels (the order in which one
+// mask yields pairs) and put right where O is read. The V rows of a last tile past the context are
+// zeros. A V group whose scale or zero is no number is stored as zeros too and noted in a mask per token,
+// and the rows that see the token get NaN in its channels: a product would spread it to rows that do not.
+// @PERF
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "kv4_attention.cuh"
+
+namespace tllm {
+
+__device__ int g_kv4p_status = 0;
+
+int kv4p_read_status(int *out) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_kv4p_status, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "cudaMemcpyFromSymbol(kv4 prefill status)");
+  const int zero = 0;
+  e = cudaMemcpyToSymbol(g_kv4p_status, &zero, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "cudaMemcpyToSymbol(kv4 prefill status)");
+  *out = v;
+  return TLLM_OK;
+}
+
+namespace kv4 {
+namespace {
+
+constexpr int BM = kPrefillRows;
+constexpr int BN = 128;
+constexpr int kPieces = BN / kPieceTokens;
+constexpr int kThreads = 512;
+constexpr int kRows = 128;      // softmax threads
+constexpr int kUnpackWarps = 8;
+static_assert(kUnpackWarps == kPieces, "a piece of a tile per unpacking warp");
+// Registers per thread: softmax, copies and UMMAs, unpacking (2 warpgroups). The launch has 128 each.
+constexpr int kRegsRows = 208, kRegsIssue = 64, kRegsUnpack = 120;
+static_assert(kRegsRows + kRegsIssue + 2 * kRegsUnpack <= 4 * 128, "register split");
+constexpr int TMEM_COLS = 512;
+constexpr int O_COL = 256;  // S buffers at columns [0, 128) and [128, 256)
+constexpr float kLazyRescaleLog2 = 8.0f;
+
+enum : int {
+  SITE_Q = 0x51,
+  SITE_RAWFULL = 0x52,
+  SITE_RAWEMPTY = 0x53,
+  SITE_KFULL = 0x54,
+  SITE_KEMPTY = 0x55,
+  SITE_VFULL = 0x56,
+  SITE_VEMPTY = 0x57,
+  SITE_SFULL = 0x58,
+  SITE_PFULL = 0x59,
+  SITE_PVDONE = 0x5a,
+  SITE_OFREE = 0x5b,
+};
+
+template <int D>
+struct Geo {
+  static constexpr int CHUNKS = D * 2 / 128;  // 128-byte swizzle spans per row
+  static constexpr int CHUNK_BYTES = BM * 128;
+  static constexpr int TILE_BYTES = CHUNKS * CHUNK_BYTES;
+  static constexpr int RAW_BYTES = kPieces * Piece<D>::BYTES;
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = TILE_BYTES;
+  static constexpr int V_OFF = K_OFF + 2 * TILE_BYTES;
+  static constexpr int RAW_OFF = V_OFF + 2 * TILE_BYTES;
+  static constexpr int BAD_OFF = RAW_OFF + 2 * RAW_BYTES;  // [2][BN] bytes: groups of V without numbers
+  static constexpr int ANY_OFF = BAD_OFF + 2 * BN;         // [2][kUnpackWarps] bytes: any in the piece
+  static constexpr int BAR_OFF = ANY_OFF + 2 * kUnpackWarps;
+  static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
+  static_assert(SMEM_BYTES <= 227 * 1024 && BAR_OFF % 8 == 0, "shared memory plan");
+};
+
+constexpr uint32_t kSwizzle128 = 2;
+
+template <int D>
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int k) {
+  const int byte = k * 32;
+  return make_sdesc(base + (byte / 128) * Geo<D>::CHUNK_BYTES + (byte % 128), 16, 8 * 128, kSwizzle128);
+}
+
+// Byte of 16-byte unit u (of 8 per 128-byte span) of a tile's row.
+__device__ __forceinline__ int unit_at(int row, int u) { return row * 128 + ((u ^ (row & 7)) << 4); }
+
+__device__ __forceinline__ uint32_t dup_low(uint32_t v) { return __byte_perm(v, v, 0x1010); }
+__device__ __forceinline__ uint32_t dup_high(uint32_t v) { return __byte_perm(v, v, 0x3232); }
+
+// The 8 codes of a word (4 in each half) to fp16 values code * s + z; x[i] holds the codes at bits 4 i of
+// both halves. A code c under the exponent of 1024 is 1024 + c (or 1024 + 16 c); the difference is exact.
+__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t s, uint32_t z, uint32_t (&x)[4]) {
+  constexpr uint32_t kExp = 0x64006400u;
+  const uint32_t hi = __byte_perm(w, 0u, 0x4341);  // the upper bytes of the halves
+  x[0] = add_half2((w & 0x000f000fu) | kExp, 0xe400e400u);                     // - 1024
+  x[1] = fma_half2((w & 0x00f000f0u) | kExp, 0x2c002c00u, 0xd400d400u);        // / 16 - 64
+  x[2] = add_half2((hi & 0x000f000fu) | kExp, 0xe400e400u);
+  x[3] = fma_half2((hi & 0x00f000f0u) | kExp, 0x2c002c00u, 0xd400d400u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = fma_half2(x[i], s, z);
+}
+
+__device__ __forceinline__ bool no_number(uint32_t half) { return (half & 0x7c00u) == 0x7c00u; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) {
+  using P = Piece<D>;
+  using G = Geo<D>;
+  constexpr int W = P::W;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
+  uint64_t *q_full = bars + 0;
+  uint64_t *raw_full = bars + 1;   // [2]
+  uint64_t *raw_empty = bars + 3;  // [2]
+  uint64_t *k_full = bars + 5;     // [2]
+  uint64_t *k_empty = bars + 7;    // [2]
+  uint64_t *v_full = bars + 9;     // [2]
+  uint64_t *v_empty = bars + 11;   // [2]
+  uint64_t *s_full = bars + 13;    // [2]
+  uint64_t *p_full = bars + 15;
+  uint64_t *pv_done = bars + 16;
+  uint64_t *o_free = bars + 17;
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 18);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+  __shared__ LineScan<kThreads, 1> s_line;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(q_full), kRows);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&raw_full[s]), 1);
+      mbar_init(smem_u32(&raw_empty[s]), kUnpackWarps);
+      mbar_init(smem_u32(&k_full[s]), kUnpackWarps);
+      mbar_init(smem_u32(&k_empty[s]), 1);
+      mbar_init(smem_u32(&v_full[s]), kUnpackWarps);
+      mbar_init(smem_u32(&v_empty[s]), 1);
+      mbar_init(smem_u32(&s_full[s]), 1);
+    }
+    mbar_init(smem_u32(p_full), kRows);
+    mbar_init(smem_u32(pv_done), 1);
+    mbar_init(smem_u32(o_free), kRows);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(tmem_holder), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  int64_t per, total;
+  scan_line<BM, BN>(a, s_line, 1, per, total, &g_kv4p_status);  // (synchronises the CTA)
+  tc_fence_after();
+  clear_rows<T, D>(a);
+  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t sQ = smem_u32(smem + G::Q_OFF);
+  const uint32_t sK = smem_u32(smem + G::K_OFF);
+  const uint32_t sV = smem_u32(smem + G::V_OFF);
+  const int worker = blockIdx.x;
+  int64_t pos = worker * per;
+  const int64_t end = min(pos + per, total);
+  if (threadIdx.x == 0) a.ws_open[worker].workers = 0;
+
+  // Every role walks the same segments; `it` counts the key tiles of all of them.
+  Segment sg;
+  bool more = pos < end && first_segment<BM, BN>(a, s_line.seq[0], s_line.off[0], end - pos, sg);
+  auto advance = [&] {
+    pos += sg.count;
+    more = next_segment<BM, BN>(a, end - pos, sg);
+  };
+  auto tiles = [&] { return sg.pl.seen > 0 ? sg.count : 0; };
+  auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+    return mbar_wait(smem_u32(bar), parity, abort_flag, &g_kv4p_status, TLLM_DEV_WAIT_TIMEOUT + site);
+  };
+
+  if (warp >= 8) {
+    // ------------------------------ unpacking ------------------------------
+    regs_dec<kRegsUnpack>();
+    const int piece = warp - 8;
+    bool ok = true;
+    uint32_t it = 0;
+    for (; more && ok; advance()) {
+      const int n = tiles();
+      for (int j = 0; j < n; ++j, ++it) {
+        const uint32_t st = it & 1, full = (it >> 1) & 1, empty = full ^ 1;
+        // Tokens of this warp's piece that are keys (the others were not loaded, or hold anything).
+        const int valid = min(max(sg.pl.seen - (sg.first + j) * BN - piece * kPieceTokens, 0), kPieceTokens);
+        const uint8_t *raw = smem + G::RAW_OFF + st * G::RAW_BYTES + piece * P::BYTES;
+        ok = __all_sync(0xffffffffu, wait(&raw_full[st], full, SITE_RAWFULL) && wait(&k_empty[st], empty, SITE_KEMPTY));
+        if (!ok) break;
+        if (valid > 0) {
+          uint8_t *tile = smem + G::K_OFF + st * G::TILE_BYTES;
+          const int cq = lane & 3;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // Eight lanes of one store phase: four units of rows t and t + 4, apart in the swizzle.
+            const int t = half * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3), row = piece * kPieceTokens + t;
+            uint32_t code[W], sc[W / 2], ze[W / 2];
+            load_words<W>(raw + P::K_CODES + t * (D / 2) + cq * (4 * W), code);
+            load_words<W / 2>(raw + P::k_scale(t, 0), sc);
+            load_words<W / 2>(raw + P::k_zero(t, 0), ze);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              uint32_t x[4];
+              unpack_word(code[w], (w & 1) ? dup_high(sc[w / 2]) : dup_low(sc[w / 2]),
+                          (w & 1) ? dup_high(ze[w / 2]) : dup_low(ze[w / 2]), x);
+              *reinterpret_cast<uint4 *>(tile + (w / 2) * G::CHUNK_BYTES + unit_at(row, 4 * (w & 1) + cq)) =
+                  make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&k_full[st]));
+
+        ok = __all_sync(0xffffffffu, wait(&v_empty[st], empty, SITE_VEMPTY));
+        if (!ok) break;
+        {
+          uint8_t *tile = smem + G::V_OFF + st * G::TILE_BYTES;
+          const int m = lane & 3;  // channels 32 g + 8 m + {0..7}
+          const int pr = ((lane >> 2) & 1) * 2 + ((lane >> 3) & 1) + ((lane >> 4) & 1) * 4;
+          const bool in0 = 2 * pr < valid, in1 = 2 * pr + 1 < valid;
+          uint32_t c0[W], c1[W], sc[W];  // [token][two groups a word]
+          const uint8_t *vp = raw + P::V_CODES + pr * D + ((2 * m) ^ P::swizzle(pr)) * P::CHUNK;
+          load_words<W>(vp, c0);
+          load_words<W>(vp + P::CHUNK, c1);
+          load_words<W>(raw + P::v_scale(2 * pr, 0), sc);
+          uint32_t bad = 0;  // bits g: token 2 pr, bits 8 + g: the next one
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
+            uint32_t s0 = (g & 1) ? sc[g / 2] >> 16 : sc[g / 2] & 0xffffu;
+            uint32_t s1 = (g & 1) ? sc[W / 2 + g / 2] >> 16 : sc[W / 2 + g / 2] & 0xffffu;
+            const uint32_t zz = *reinterpret_cast<const uint32_t *>(raw + P::v_zero(2 * pr, g));
+            uint32_t z0 = zz & 0xffffu, z1 = zz >> 16;
+            if (!in0) s0 = z0 = 0;
+            if (!in1) s1 = z1 = 0;
+            if (no_number(s0) || no_number(z0)) {
+              bad |= 1u << g;
+              s0 = z0 = 0;
+            }
+            if (no_number(s1) || no_number(z1)) {
+              bad |= 256u << g;
+              s1 = z1 = 0;
+            }
+            const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+            const int unit = 4 * (g & 1) + m, row = piece * kPieceTokens + 2 * pr;
+            uint8_t *chunk = tile + (g / 2) * G::CHUNK_BYTES;
+            uint32_t x[4];
+            unpack_word(__byte_perm(c0[g / 2], c1[g / 2], sel), dup_low(s0), dup_low(z0), x);
+            *reinterpret_cast<uint4 *>(chunk + unit_at(row, unit)) = make_uint4(x[0], x[1], x[2], x[3]);
+            unpack_word(__byte_perm(c0[W / 2 + g / 2], c1[W / 2 + g / 2], sel), dup_low(s1), dup_low(z1), x);
+            *reinterpret_cast<uint4 *>(chunk + unit_at(row + 1, unit)) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+          if (m == 0)
+            *reinterpret_cast<uint16_t *>(smem + G::BAD_OFF + st * BN + piece * kPieceTokens + 2 * pr) = static_cast<uint16_t>(bad);
+          const bool any = __any_sync(0xffffffffu, bad != 0);
+          if (lane == 0) smem[G::ANY_OFF + st * kUnpackWarps + piece] = any;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&v_full[st]));
+          mbar_arrive(smem_u32(&raw_empty[st]));
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    regs_dec<kRegsIssue>();
+    if (warp == 5) {
+      // ------------------------------ copies ------------------------------
+      const int per_page = (1 << a.log2_bs) / kPieceTokens;
+      bool ok = true;
+      uint32_t it = 0;
+      for (; more && ok; advance()) {
+        const int n = tiles();
+        const int32_t *bt = a.block_tables + sg.pl.b * a.sbt0;
+        // Lane i: page i of a tile, read one tile ahead.
+        auto page_of = [&](int j) -> int {
+          const int tok = (sg.first + j) * BN + (lane << a.log2_bs);
+          if (j >= n || (lane << a.log2_bs) >= BN || tok >= sg.pl.seen) return -1;
+          const int p = __ldg(bt + static_cast<int64_t>(tok >> a.log2_bs) * a.sbt1);
+          if (p >= 0 && p < a.num_blocks) return p;
+          atomicCAS(&g_kv4p_status, 0, TLLM_DEV_BAD_INDEX);
+          return 0;
+        };
+        int page = page_of(0);
+        for (int j = 0; j < n; ++j, ++it) {
+          const uint32_t st = it & 1;
+          const int here = page;
+          page = page_of(j + 1);
+          ok = __all_sync(0xffffffffu, wait(&raw_empty[st], ((it >> 1) & 1) ^ 1, SITE_RAWEMPTY));
+          if (!ok) break;
+          const int pieces = min((sg.pl.seen - (sg.first + j) * BN + kPieceTokens - 1) / kPieceTokens, kPieces);
+          const uint32_t bar = smem_u32(&raw_full[st]);
+          if (lane == 0) mbar_arrive_expect_tx(bar, pieces * P::BYTES);
+          __syncwarp();
+          if (here >= 0) {
+            const int at = lane * per_page;  // the page's first piece in the tile
+            bulk_load(smem_u32(smem + G::RAW_OFF) + st * G::RAW_BYTES + at * P::BYTES,
+                      a.cache + static_cast<int64_t>(here) * a.sblk + sg.hk * a.shead,
+                      min(per_page, pieces - at) * P::BYTES, bar);
+          }
+        }
+      }
+      if (!ok) {
+        // The copies in flight still write to this CTA's memory: give them their time.
+        for (uint32_t i = it > 2 ? it - 2 : 0; i < it; ++i) {
+          const long long since = clock64();
+          while (!mbar_try_wait(smem_u32(&raw_full[i & 1]), (i >> 1) & 1) && clock64() - since < kWaitLimitCycles) {
+          }
+        }
+      }
+    } else if (warp == 4 && lane == 0) {
+      // ------------------------------ UMMAs ------------------------------
+      const uint32_t idesc_qk = make_idesc_f16(BM, BN, false, false, false);
+      const uint32_t idesc_pv = make_idesc_f16(BM, D, false, false, true);
+      bool ok = true;
+      uint32_t it = 0, seg = 0;
+      for (; more && ok; advance()) {
+        const int n = tiles();
+        if (n == 0) continue;
+        auto issue_qk = [&](uint32_t i) {
+          const uint32_t kbase = sK + (i & 1) * G::TILE_BYTES;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16_ss(tmem_base + (i & 1) * BN, kmajor_desc<D>(sQ, k), kmajor_desc<D>(kbase, k), idesc_qk,
+                        k != 0 ? 1u : 0u);
+          umma_commit(smem_u32(&s_full[i & 1]));
+          umma_commit(smem_u32(&k_empty[i & 1]));
+        };
+        auto next_qk = [&](uint32_t i) {
+          ok = wait(&k_full[i & 1], (i >> 1) & 1, SITE_KFULL);
+          if (!ok) return;
+          tc_fence_after();
+          issue_qk(i);
+        };
+        ok = wait(q_full, seg & 1, SITE_Q);
+        for (int j = 0; j < 2 && j < n && ok; ++j) next_qk(it + j);
+        for (int j = 0; j < n && ok; ++j, ++it) {
+          const uint32_t st = it & 1;
+          ok = wait(p_full, it & 1, SITE_PFULL) && wait(&v_full[st], (it >> 1) & 1, SITE_VFULL) &&
+               (j > 0 || seg == 0 || wait(o_free, (seg - 1) & 1, SITE_OFREE));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vbase = sV + st * G::TILE_BYTES;
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            umma_f16_ts(tmem_base + O_COL, tmem_base + st * BN + k * 8,
+                        make_sdesc(vbase + k * 16 * 128, G::CHUNK_BYTES, 8 * 128, kSwizzle128), idesc_pv,
+                        (j | k) != 0 ? 1u : 0u);
+          umma_commit(smem_u32(&v_empty[st]));
+          umma_commit(smem_u32(pv_done));
+          // Its S buffer is this tile's, rewritten only after the P V above (one pipe, in order).
+          if (j + 2 < n) next_qk(it + 2);
+        }
+        ++seg;
+      }
+    }
+  } else {
+    // ------------------------------ rows ------------------------------
+    regs_inc<kRegsRows>();
+    const int row = threadIdx.x;  // = TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t o_tm = tmem_base + lane_off + O_COL;
+    // A scale of 0 is a zero q (a hidden score is -infinity, which a factor of 0 would spoil).
+    const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+    const float sign = a.scale_log2 > 0.f ? 1.f : (a.scale_log2 < 0.f ? -1.f : 0.f);
+    // Brings the segment's q row into shared memory; returns the factor of its scores.
+    auto load_q = [&]() -> float {
+      uint4 raw[D / 8];
+      const bool in = row < sg.pl.nr;
+      const int rr = sg.pl.r0 + row;
+      const T *q = static_cast<const T *>(a.q) + (sg.pl.row0 + rr / a.G) * a.sq0 + (sg.hk * a.G + rr % a.G) * a.sq1;
+      float top = 0.f;
+#pragma unroll
+      for (int u = 0; u < D / 8; ++u) raw[u] = in ? __ldg(reinterpret_cast<const uint4 *>(q) + u) : make_uint4(0, 0, 0, 0);
+      float up = sign, down = scale;
+      if constexpr (kBF16) {
+#pragma unroll
+        for (int u = 0; u < D / 8; ++u) {
+          const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Pack2<T>::unpack(w[i]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const int e = max((__float_as_int(top) >> 23) - 127, -100);
+        up = pow2(12 - e) * sign;
+        down = pow2(e) * (scale / 4096.f);
+      }
+#pragma unroll
+      for (int u = 0; u < D / 8; ++u) {
+        uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = Pack2<T>::unpack(w[i]);
+          w[i] = pack_half(f.x * up, f.y * up);
+        }
+        *reinterpret_cast<uint4 *>(smem + G::Q_OFF + (u / 8) * G::CHUNK_BYTES + unit_at(row, u % 8)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(q_full));
+      return down;
+    };
+    bool ok = true, at_start = true;
+    uint32_t it = 0;
+    float rs = more && tiles() > 0 ? load_q() : 0.f;
+    while (more && ok) {
+      const int n = tiles();
+      const int keys = row < sg.pl.nr ? row_keys(a, sg.pl, sg.pl.r0 + row) : 0;
+      float m_use = -INFINITY, l_run = 0.f;
+      uint32_t bad = 0;  // groups of V without numbers that the row sees
+      for (int j = 0; j < n; ++j, ++it) {
+        const uint32_t sb = it & 1;
+        ok = __all_sync(0xffffffffu, wait(&s_full[sb], (it >> 1) & 1, SITE_SFULL));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_tm = tmem_base + lane_off + sb * BN;
+        const int k0 = (sg.first + j) * BN;
+        uint32_t sr[BN];
+        tmem_ld4x32(s_tm, sr);
+        if (k0 + BN > keys) {
+#pragma unroll
+          for (int t = 0; t < BN; ++t)
+            if (k0 + t >= keys) sr[t] = __float_as_uint(-INFINITY);
+        }
+        float mx8[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) mx8[t] = __uint_as_float(sr[t]);
+#pragma unroll
+        for (int t = 8; t < BN; t += 2)
+          mx8[(t >> 1) & 7] = max3f(mx8[(t >> 1) & 7], __uint_as_float(sr[t]), __uint_as_float(sr[t + 1]));
+        const float mx = rs * max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+        // O is stable once the previous tile's P V has completed.
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, wait(pv_done, (it - 1) & 1, SITE_PVDONE));
+          if (!ok) break;
+        }
+        float alpha = 1.0f;
+        bool rescale = false;
+        if (m_use == -INFINITY) {
+          m_use = mx;  // nothing accumulated yet (every earlier P of this row was 0)
+        } else if (mx > m_use + kLazyRescaleLog2) {
+          alpha = ex2_approx(m_use - mx);
+          m_use = mx;
+          rescale = true;
+        }
+        const float neg_m = m_use == -INFINITY ? 0.f : -m_use;
+        // The exponents below are exact products less the rounded maximum, which is within half an ulp of
+        // its own product; where half an ulp could be many units, round the products first.
+        float factor = rs;
+        if (__any_sync(0xffffffffu, fabsf(m_use) >= 268435456.f && m_use != -INFINITY)) {
+#pragma unroll
+          for (int t = 0; t < BN; ++t) sr[t] = __float_as_uint(__uint_as_float(sr[t]) * rs);
+          factor = 1.f;
+        }
+        const uint64_t scale2 = f2_pack(factor, factor);
+        const uint64_t negm2 = f2_pack(neg_m, neg_m);
+        uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int t = 0; t < 64; t += 2) {
+            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sr[64 * hlf + t]), __uint_as_float(sr[64 * hlf + t + 1])), scale2, negm2);
+            float x0, x1;
+            f2_unpack(x2, x0, x1);
+            const float p0 = ex2_approx(x0);
+            const float p1 = ex2_approx(x1);
+            ps2[(t >> 1) & 3] = f2_add(ps2[(t >> 1) & 3], f2_pack(p0, p1));
+            pk[t >> 1] = pack_half(p0, p1);
+          }
+          tmem_st32(s_tm + 32 * hlf, pk);
+        }
+        float ps[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f2_unpack(ps2[i], ps[2 * i], ps[2 * i + 1]);
+        l_run = l_run * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(o_tm + c, r);
+#pragma unroll
+            for (int t = 0; t < 32; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
+            tmem_st32(o_tm + c, r);
+          }
+        }
+        // V's groups without numbers: the notes are overwritten only after this tile's P V.
+        ok = __all_sync(0xffffffffu, wait(&v_full[sb], (it >> 1) & 1, SITE_VFULL));
+        if (!ok) break;
+        if (*reinterpret_cast<const volatile uint64_t *>(smem + G::ANY_OFF + sb * kUnpackWarps) != 0)
+          for (int t = 0; t < BN && k0 + t < keys; ++t) bad |= smem[G::BAD_OFF + sb * BN + t];
+        tc_fence_before();
+        mbar_arrive(smem_u32(p_full));
+      }
+      if (!ok) break;
+      // ---- the next segment's q goes in first: this one's products with Q are complete ----
+      const Segment done = sg;
+      const int64_t done_pos = pos;
+      const float done_m = m_use, done_l = l_run;
+      advance();
+      if (more && tiles() > 0) rs = load_q();
+      // ---- results ----
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, wait(pv_done, (it - 1) & 1, SITE_PVDONE));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool whole = done.count == done.nt, in = row < done.pl.nr;
+      const int64_t slot = (2 * static_cast<int64_t>(worker) + (at_start ? 0 : 1)) * BM + row;
+      const int rr = done.pl.r0 + row;
+      const float inv = 1.f / done_l;  // no key: 0 / 0
+      T *o = static_cast<T *>(a.o) + (done.pl.row0 + rr / a.G) * a.so0 + (done.hk * a.G + rr % a.G) * a.so1;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld32(o_tm + c, r);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 32; ++t) r[t] = 0u;
+        }
+        if (bad & (1u << (c / 32))) {
+#pragma unroll
+          for (int t = 0; t < 32; ++t) r[t] = 0x7fc00000u;  // NaN
+        }
+        if (!in) continue;
+#pragma unroll
+        for (int t = 0; t < 32; t += 8) {
+          float v[8];  // columns 2 i + h hold channels i + 4 h
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[(i >> 1) + 4 * (i & 1)] = __uint_as_float(r[t + i]);
+          if (whole) {
+            uint4 pk;
+            pk.x = Pack2<T>::pack(v[0] * inv, v[1] * inv);
+            pk.y = Pack2<T>::pack(v[2] * inv, v[3] * inv);
+            pk.z = Pack2<T>::pack(v[4] * inv, v[5] * inv);
+            pk.w = Pack2<T>::pack(v[6] * inv, v[7] * inv);
+            *reinterpret_cast<uint4 *>(o + c + t) = pk;
+          } else {
+            float4 *p = reinterpret_cast<float4 *>(a.ws_acc + slot * D + c + t);
+            p[0] = make_float4(v[0], v[1], v[2], v[3]);
+            p[1] = make_float4(v[4], v[5], v[6], v[7]);
+          }
+        }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        mbar_arrive(smem_u32(o_free));
+      }
+      if (!whole && in) a.ws_ml[slot] = make_float2(done_l == 0.f ? -INFINITY : (done_m == -INFINITY ? 0.f : done_m), done_l);
+      if (!whole && done.first == 0 && row == 0)
+        a.ws_open[worker] = Open{static_cast<int>((done_pos + done.nt - 1) / per) - worker + 1,
+                                 2 * worker + (at_start ? 0 : 1), done.hk, done.pl.row0, done.pl.r0, done.pl.nr, 0, 0};
+      at_start = false;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+template <typename T, int D>
+int launch(const Args &a, cudaStream_t st) {
+  auto kern = kv4_prefill_kernel<T, D>;
+  KernelLaunchInfo info;
+  const int rc = prepare_kernel(reinterpret_cast<const void *>(kern), Geo<D>::SMEM_BYTES, kThreads, 1, &info);
+  if (rc) return rc;
+  if (info.num_regs * kThreads < 128 * (kRegsRows + kRegsIssue + 2 * kRegsUnpack))
+    return fail(TLLM_ERR_CUDA, "paged kv4 prefill: built with %d registers per thread, the split needs more", info.num_regs);
+  kern<<<a.workers, kThreads, Geo<D>::SMEM_BYTES, st>>>(a);
+  return cuda_status(cudaGetLastError(), "paged kv4 prefill launch");
+}
+
+}  // namespace
+
+int launch_prefill(const Args &a, int64_t D, int dtype, cudaStream_t st) {
+  if (dtype == TLLM_DTYPE_F16) return D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+  return D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
+}
+
+}  // namespace kv4
+}  // namespace tllm
