@@ -2,15 +2,15 @@
 // tiles of 128 query rows and 128 keys, the keys and values brought to fp16 on the way.
 //
 // A worker of the line (kv4_attention.cuh) is a CTA, one per SM; row tiles have 128 rows, key tiles
-// 128 keys. Work goes through rings of two stages:
-//   warp 5        copies: the tile's pages, K and V of one head, by bulk copies into the raw ring
+// 128 keys. Work goes through rings:
+//   warp 17       copies: the tile's pages, K and V of one head, by bulk copies into the raw ring
 //   warps 8-15    unpack, a piece of 16 tokens each: code * scale + zero in fp16 (11 bits: an error of
 //                 2^-12 of a value against the half step of 1/30 of its group's range that 4 bits
 //                 cost), stored swizzled as the K and V operands
-//   warp 4        TMEM allocation and the lane that issues the UMMAs: S = Q K^T into one of two TMEM
+//   warp 16       TMEM allocation and the lane that issues the UMMAs: S = Q K^T into one of two TMEM
 //                 buffers (the next tile's overlaps this tile's softmax), O += P V with P from TMEM
-//   warps 0-3     one query row per thread: q to fp16 (bf16 rows by a power of two that keeps them in
-//                 its range), softmax with a lazy rescale of O (2^8), the results
+//   warps 0-7     two threads per query row, 64 keys of a tile each: q to fp16 (bf16 rows by a power of
+//                 two that keeps them in its range), softmax with a lazy rescale of O (2^8), results
 // V's columns are stored in the order 0 4 1 5 2 6 3 7 of every eight channels (the order in which one
 // mask yields pairs) and put right where O is read. The V rows of a last tile past the context are
 // zeros. A V group whose scale or zero is no number is stored as zeros too and noted in a mask per token,
@@ -44,15 +44,16 @@ namespace {
 constexpr int BM = kPrefillRows;
 constexpr int BN = 128;
 constexpr int kPieces = BN / kPieceTokens;
-constexpr int kThreads = 512;
-constexpr int kRows = 128;      // softmax threads
+constexpr int kRowThreads = 256;  // two per query row
+constexpr int kHalf = BN / 2;     // keys of a tile per thread of a row
 constexpr int kUnpackWarps = 8;
+constexpr int kRawStages = 3;     // tiles of the cache on their way or being unpacked (shared memory holds no more)
+constexpr int kUmmaWarp = 16, kCopyWarp = 17;
+constexpr int kThreads = 18 * 32;
 static_assert(kUnpackWarps == kPieces, "a piece of a tile per unpacking warp");
-// Registers per thread: softmax, copies and UMMAs, unpacking (2 warpgroups). The launch has 128 each.
-constexpr int kRegsRows = 208, kRegsIssue = 64, kRegsUnpack = 120;
-static_assert(kRegsRows + kRegsIssue + 2 * kRegsUnpack <= 4 * 128, "register split");
 constexpr int TMEM_COLS = 512;
 constexpr int O_COL = 256;  // S buffers at columns [0, 128) and [128, 256)
+constexpr int P_COL = 384;  // P buffers at columns [384, 448) and [448, 512)
 constexpr float kLazyRescaleLog2 = 8.0f;
 
 enum : int {
@@ -67,6 +68,8 @@ enum : int {
   SITE_PFULL = 0x59,
   SITE_PVDONE = 0x5a,
   SITE_OFREE = 0x5b,
+  SITE_SEMPTY = 0x5c,
+  SITE_PAIR = 0x5d,
 };
 
 template <int D>
@@ -79,9 +82,10 @@ struct Geo {
   static constexpr int K_OFF = TILE_BYTES;
   static constexpr int V_OFF = K_OFF + 2 * TILE_BYTES;
   static constexpr int RAW_OFF = V_OFF + 2 * TILE_BYTES;
-  static constexpr int BAD_OFF = RAW_OFF + 2 * RAW_BYTES;  // [2][BN] bytes: groups of V without numbers
+  static constexpr int BAD_OFF = RAW_OFF + kRawStages * RAW_BYTES;  // [2][BN] bytes: groups of V without numbers
   static constexpr int ANY_OFF = BAD_OFF + 2 * BN;         // [2][kUnpackWarps] bytes: any in the piece
-  static constexpr int BAR_OFF = ANY_OFF + 2 * kUnpackWarps;
+  static constexpr int MAX_OFF = ANY_OFF + 2 * kUnpackWarps;  // [2][2][BM] floats between a row's threads
+  static constexpr int BAR_OFF = MAX_OFF + 4 * BM * 4;
   static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024 && BAR_OFF % 8 == 0, "shared memory plan");
 };
@@ -97,8 +101,12 @@ __device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int k) {
 // Byte of 16-byte unit u (of 8 per 128-byte span) of a tile's row.
 __device__ __forceinline__ int unit_at(int row, int u) { return row * 128 + ((u ^ (row & 7)) << 4); }
 
-__device__ __forceinline__ uint32_t dup_low(uint32_t v) { return __byte_perm(v, v, 0x1010); }
-__device__ __forceinline__ uint32_t dup_high(uint32_t v) { return __byte_perm(v, v, 0x3232); }
+// One half of a word in both (the compiler takes it as an operand's modifier).
+__device__ __forceinline__ uint32_t twice(uint32_t v, bool high) {
+  const __half2 h = *reinterpret_cast<const __half2 *>(&v);
+  const __half2 r = high ? __high2half2(h) : __low2half2(h);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
 
 // The 8 codes of a word (4 in each half) to fp16 values code * s + z; x[i] holds the codes at bits 4 i of
 // both halves. A code c under the exponent of 1024 is 1024 + c (or 1024 + 16 c); the difference is exact.
@@ -113,8 +121,6 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t s, uint32_t z, 
   for (int i = 0; i < 4; ++i) x[i] = fma_half2(x[i], s, z);
 }
 
-__device__ __forceinline__ bool no_number(uint32_t half) { return (half & 0x7c00u) == 0x7c00u; }
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) {
   using P = Piece<D>;
@@ -125,17 +131,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
   uint64_t *q_full = bars + 0;
-  uint64_t *raw_full = bars + 1;   // [2]
-  uint64_t *raw_empty = bars + 3;  // [2]
-  uint64_t *k_full = bars + 5;     // [2]
-  uint64_t *k_empty = bars + 7;    // [2]
-  uint64_t *v_full = bars + 9;     // [2]
-  uint64_t *v_empty = bars + 11;   // [2]
-  uint64_t *s_full = bars + 13;    // [2]
-  uint64_t *p_full = bars + 15;
-  uint64_t *pv_done = bars + 16;
-  uint64_t *o_free = bars + 17;
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 18);
+  uint64_t *k_full = bars + 1;     // [2]
+  uint64_t *k_empty = bars + 3;    // [2]
+  uint64_t *v_full = bars + 5;     // [2]
+  uint64_t *v_empty = bars + 7;    // [2]
+  uint64_t *s_full = bars + 9;     // [2]
+  uint64_t *p_full = bars + 11;
+  uint64_t *pv_done = bars + 12;   // [2], as s_full by the tile's parity
+  uint64_t *o_free = bars + 14;
+  uint64_t *s_empty = bars + 15;   // [2]
+  uint64_t *pair = bars + 17;      // [4]
+  uint64_t *raw_full = bars + 21;                // [kRawStages]
+  uint64_t *raw_empty = raw_full + kRawStages;   // [kRawStages]
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(raw_empty + kRawStages);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   __shared__ LineScan<kThreads, 1> s_line;
 
@@ -143,23 +151,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(q_full), kRows);
+    mbar_init(smem_u32(q_full), kRowThreads);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(smem_u32(&raw_full[s]), 1);
-      mbar_init(smem_u32(&raw_empty[s]), kUnpackWarps);
       mbar_init(smem_u32(&k_full[s]), kUnpackWarps);
       mbar_init(smem_u32(&k_empty[s]), 1);
       mbar_init(smem_u32(&v_full[s]), kUnpackWarps);
       mbar_init(smem_u32(&v_empty[s]), 1);
       mbar_init(smem_u32(&s_full[s]), 1);
+      mbar_init(smem_u32(&s_empty[s]), kRowThreads);
+      mbar_init(smem_u32(&pv_done[s]), 1);
     }
-    mbar_init(smem_u32(p_full), kRows);
-    mbar_init(smem_u32(pv_done), 1);
-    mbar_init(smem_u32(o_free), kRows);
+    for (int s = 0; s < kRawStages; ++s) {
+      mbar_init(smem_u32(&raw_full[s]), 1);
+      mbar_init(smem_u32(&raw_empty[s]), kUnpackWarps);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(smem_u32(&pair[s]), 64);
+    mbar_init(smem_u32(p_full), kRowThreads);
+    mbar_init(smem_u32(o_free), kRowThreads);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 4) {
+  if (warp == kUmmaWarp) {
     tmem_alloc(smem_u32(tmem_holder), TMEM_COLS);
     tmem_relinquish();
   }
@@ -189,20 +201,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
     return mbar_wait(smem_u32(bar), parity, abort_flag, &g_kv4p_status, TLLM_DEV_WAIT_TIMEOUT + site);
   };
 
-  if (warp >= 8) {
+  if (warp >= 8 && warp < 8 + kUnpackWarps) {
     // ------------------------------ unpacking ------------------------------
-    regs_dec<kRegsUnpack>();
     const int piece = warp - 8;
     bool ok = true;
     uint32_t it = 0;
     for (; more && ok; advance()) {
       const int n = tiles();
       for (int j = 0; j < n; ++j, ++it) {
-        const uint32_t st = it & 1, full = (it >> 1) & 1, empty = full ^ 1;
+        const uint32_t st = it & 1, empty = ((it >> 1) & 1) ^ 1, rst = it % kRawStages;
         // Tokens of this warp's piece that are keys (the others were not loaded, or hold anything).
         const int valid = min(max(sg.pl.seen - (sg.first + j) * BN - piece * kPieceTokens, 0), kPieceTokens);
-        const uint8_t *raw = smem + G::RAW_OFF + st * G::RAW_BYTES + piece * P::BYTES;
-        ok = __all_sync(0xffffffffu, wait(&raw_full[st], full, SITE_RAWFULL) && wait(&k_empty[st], empty, SITE_KEMPTY));
+        const uint8_t *raw = smem + G::RAW_OFF + rst * G::RAW_BYTES + piece * P::BYTES;
+        ok = __all_sync(0xffffffffu, wait(&raw_full[rst], (it / kRawStages) & 1, SITE_RAWFULL) && wait(&k_empty[st], empty, SITE_KEMPTY));
         if (!ok) break;
         if (valid > 0) {
           uint8_t *tile = smem + G::K_OFF + st * G::TILE_BYTES;
@@ -218,8 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
 #pragma unroll
             for (int w = 0; w < W; ++w) {
               uint32_t x[4];
-              unpack_word(code[w], (w & 1) ? dup_high(sc[w / 2]) : dup_low(sc[w / 2]),
-                          (w & 1) ? dup_high(ze[w / 2]) : dup_low(ze[w / 2]), x);
+              unpack_word(code[w], twice(sc[w / 2], w & 1), twice(ze[w / 2], w & 1), x);
               *reinterpret_cast<uint4 *>(tile + (w / 2) * G::CHUNK_BYTES + unit_at(row, 4 * (w & 1) + cq)) =
                   make_uint4(x[0], x[1], x[2], x[3]);
             }
@@ -235,54 +245,64 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           uint8_t *tile = smem + G::V_OFF + st * G::TILE_BYTES;
           const int m = lane & 3;  // channels 32 g + 8 m + {0..7}
           const int pr = ((lane >> 2) & 1) * 2 + ((lane >> 3) & 1) + ((lane >> 4) & 1) * 4;
-          const bool in0 = 2 * pr < valid, in1 = 2 * pr + 1 < valid;
-          uint32_t c0[W], c1[W], sc[W];  // [token][two groups a word]
+          uint32_t c0[W], c1[W], sc[W], ze[W];  // [token][two groups a word], [token][..], zeros [group]: two tokens
           const uint8_t *vp = raw + P::V_CODES + pr * D + ((2 * m) ^ P::swizzle(pr)) * P::CHUNK;
           load_words<W>(vp, c0);
           load_words<W>(vp + P::CHUNK, c1);
           load_words<W>(raw + P::v_scale(2 * pr, 0), sc);
-          uint32_t bad = 0;  // bits g: token 2 pr, bits 8 + g: the next one
+          uint32_t big = 0;
 #pragma unroll
           for (int g = 0; g < W; ++g) {
-            uint32_t s0 = (g & 1) ? sc[g / 2] >> 16 : sc[g / 2] & 0xffffu;
-            uint32_t s1 = (g & 1) ? sc[W / 2 + g / 2] >> 16 : sc[W / 2 + g / 2] & 0xffffu;
-            const uint32_t zz = *reinterpret_cast<const uint32_t *>(raw + P::v_zero(2 * pr, g));
-            uint32_t z0 = zz & 0xffffu, z1 = zz >> 16;
-            if (!in0) s0 = z0 = 0;
-            if (!in1) s1 = z1 = 0;
-            if (no_number(s0) || no_number(z0)) {
-              bad |= 1u << g;
-              s0 = z0 = 0;
-            }
-            if (no_number(s1) || no_number(z1)) {
-              bad |= 256u << g;
-              s1 = z1 = 0;
-            }
+            ze[g] = *reinterpret_cast<const uint32_t *>(raw + P::v_zero(2 * pr, g));
+            big = __vmaxu2(big, __vmaxu2(sc[g] & 0x7fff7fffu, ze[g] & 0x7fff7fffu));
+          }
+          // Tokens past the last key, or some value that is no number: zeros, and a note of the latter.
+          uint32_t bad = 0;  // bits g: token 2 pr, bits 8 + g: the next one
+          const bool odd = valid < kPieceTokens || max(big & 0xffffu, big >> 16) >= 0x7c00u;
+          const bool any_odd = __any_sync(0xffffffffu, odd);
+          if (any_odd) {
+#pragma unroll
+            for (int g = 0; g < W; ++g)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int sh_s = 16 * (g & 1), sh_z = 16 * e;
+                const uint32_t s1 = (sc[e * (W / 2) + g / 2] >> sh_s) & 0x7fffu, z1 = (ze[g] >> sh_z) & 0x7fffu;
+                const bool past = 2 * pr + e >= valid, none = s1 >= 0x7c00u || z1 >= 0x7c00u;
+                if (!past && none) bad |= 1u << (8 * e + g);
+                if (past || none) {
+                  sc[e * (W / 2) + g / 2] &= ~(0xffffu << sh_s);
+                  ze[g] &= ~(0xffffu << sh_z);
+                }
+              }
+          }
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
             const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
             const int unit = 4 * (g & 1) + m, row = piece * kPieceTokens + 2 * pr;
             uint8_t *chunk = tile + (g / 2) * G::CHUNK_BYTES;
-            uint32_t x[4];
-            unpack_word(__byte_perm(c0[g / 2], c1[g / 2], sel), dup_low(s0), dup_low(z0), x);
-            *reinterpret_cast<uint4 *>(chunk + unit_at(row, unit)) = make_uint4(x[0], x[1], x[2], x[3]);
-            unpack_word(__byte_perm(c0[W / 2 + g / 2], c1[W / 2 + g / 2], sel), dup_low(s1), dup_low(z1), x);
-            *reinterpret_cast<uint4 *>(chunk + unit_at(row + 1, unit)) = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t x[4];
+              unpack_word(__byte_perm(c0[e * (W / 2) + g / 2], c1[e * (W / 2) + g / 2], sel),
+                          twice(sc[e * (W / 2) + g / 2], g & 1), twice(ze[g], e), x);
+              *reinterpret_cast<uint4 *>(chunk + unit_at(row + e, unit)) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
           }
-          if (m == 0)
+          const bool any = any_odd && __any_sync(0xffffffffu, bad != 0);
+          if (any && m == 0)
             *reinterpret_cast<uint16_t *>(smem + G::BAD_OFF + st * BN + piece * kPieceTokens + 2 * pr) = static_cast<uint16_t>(bad);
-          const bool any = __any_sync(0xffffffffu, bad != 0);
           if (lane == 0) smem[G::ANY_OFF + st * kUnpackWarps + piece] = any;
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(smem_u32(&v_full[st]));
-          mbar_arrive(smem_u32(&raw_empty[st]));
+          mbar_arrive(smem_u32(&raw_empty[rst]));
         }
       }
     }
-  } else if (warp >= 4) {
-    regs_dec<kRegsIssue>();
-    if (warp == 5) {
+  } else if (warp >= 8) {
+    if (warp == kCopyWarp) {
       // ------------------------------ copies ------------------------------
       const int per_page = (1 << a.log2_bs) / kPieceTokens;
       bool ok = true;
@@ -301,10 +321,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         };
         int page = page_of(0);
         for (int j = 0; j < n; ++j, ++it) {
-          const uint32_t st = it & 1;
+          const uint32_t st = it % kRawStages;
           const int here = page;
           page = page_of(j + 1);
-          ok = __all_sync(0xffffffffu, wait(&raw_empty[st], ((it >> 1) & 1) ^ 1, SITE_RAWEMPTY));
+          ok = __all_sync(0xffffffffu, wait(&raw_empty[st], ((it / kRawStages) & 1) ^ 1, SITE_RAWEMPTY));
           if (!ok) break;
           const int pieces = min((sg.pl.seen - (sg.first + j) * BN + kPieceTokens - 1) / kPieceTokens, kPieces);
           const uint32_t bar = smem_u32(&raw_full[st]);
@@ -320,13 +340,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
       }
       if (!ok) {
         // The copies in flight still write to this CTA's memory: give them their time.
-        for (uint32_t i = it > 2 ? it - 2 : 0; i < it; ++i) {
+        for (uint32_t i = it > kRawStages ? it - kRawStages : 0; i < it; ++i) {
           const long long since = clock64();
-          while (!mbar_try_wait(smem_u32(&raw_full[i & 1]), (i >> 1) & 1) && clock64() - since < kWaitLimitCycles) {
+          while (!mbar_try_wait(smem_u32(&raw_full[i % kRawStages]), (i / kRawStages) & 1) && clock64() - since < kWaitLimitCycles) {
           }
         }
       }
-    } else if (warp == 4 && lane == 0) {
+    } else if (lane == 0) {
       // ------------------------------ UMMAs ------------------------------
       const uint32_t idesc_qk = make_idesc_f16(BM, BN, false, false, false);
       const uint32_t idesc_pv = make_idesc_f16(BM, D, false, false, true);
@@ -345,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           umma_commit(smem_u32(&k_empty[i & 1]));
         };
         auto next_qk = [&](uint32_t i) {
-          ok = wait(&k_full[i & 1], (i >> 1) & 1, SITE_KFULL);
+          ok = wait(&k_full[i & 1], (i >> 1) & 1, SITE_KFULL) && wait(&s_empty[i & 1], ((i >> 1) & 1) ^ 1, SITE_SEMPTY);
           if (!ok) return;
           tc_fence_after();
           issue_qk(i);
@@ -361,12 +381,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           const uint32_t vbase = sV + st * G::TILE_BYTES;
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            umma_f16_ts(tmem_base + O_COL, tmem_base + st * BN + k * 8,
+            umma_f16_ts(tmem_base + O_COL, tmem_base + P_COL + st * kHalf + k * 8,
                         make_sdesc(vbase + k * 16 * 128, G::CHUNK_BYTES, 8 * 128, kSwizzle128), idesc_pv,
                         (j | k) != 0 ? 1u : 0u);
           umma_commit(smem_u32(&v_empty[st]));
-          umma_commit(smem_u32(pv_done));
-          // Its S buffer is this tile's, rewritten only after the P V above (one pipe, in order).
+          umma_commit(smem_u32(&pv_done[st]));
           if (j + 2 < n) next_qk(it + 2);
         }
         ++seg;
@@ -374,46 +393,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
     }
   } else {
     // ------------------------------ rows ------------------------------
-    regs_inc<kRegsRows>();
-    const int row = threadIdx.x;  // = TMEM lane
-    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad ..., keys 64 half ...
+    const int row = quad * 32 + lane;             // = TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t o_tm = tmem_base + lane_off + O_COL;
+    float *s_max = reinterpret_cast<float *>(smem + G::MAX_OFF);
+    // A number from each of the row's two threads to the other: warps quad and quad + 4 meet. (On a
+    // barrier whose wait is bounded; after one that gave up, the next wait for work leaves.)
+    uint32_t meets = 0;
+    auto other = [&](float v) -> float {
+      float *at = s_max + (meets & 1) * 2 * BM;
+      at[half * BM + row] = v;
+      mbar_arrive(smem_u32(&pair[quad]));
+      wait(&pair[quad], meets & 1, SITE_PAIR);
+      ++meets;
+      return at[(half ^ 1) * BM + row];
+    };
     // A scale of 0 is a zero q (a hidden score is -infinity, which a factor of 0 would spoil).
     const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
     const float sign = a.scale_log2 > 0.f ? 1.f : (a.scale_log2 < 0.f ? -1.f : 0.f);
-    // Brings the segment's q row into shared memory; returns the factor of its scores.
+    // Brings this thread's half of the segment's q row into shared memory; returns the factor of its scores.
+    constexpr int kUnits = D / 16;
     auto load_q = [&]() -> float {
-      uint4 raw[D / 8];
+      uint4 raw[kUnits];
       const bool in = row < sg.pl.nr;
       const int rr = sg.pl.r0 + row;
-      const T *q = static_cast<const T *>(a.q) + (sg.pl.row0 + rr / a.G) * a.sq0 + (sg.hk * a.G + rr % a.G) * a.sq1;
-      float top = 0.f;
+      const T *q = static_cast<const T *>(a.q) + (sg.pl.row0 + rr / a.G) * a.sq0 + (sg.hk * a.G + rr % a.G) * a.sq1 + half * (D / 2);
 #pragma unroll
-      for (int u = 0; u < D / 8; ++u) raw[u] = in ? __ldg(reinterpret_cast<const uint4 *>(q) + u) : make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < kUnits; ++u) raw[u] = in ? __ldg(reinterpret_cast<const uint4 *>(q) + u) : make_uint4(0, 0, 0, 0);
       float up = sign, down = scale;
       if constexpr (kBF16) {
+        uint32_t big = 0;  // the exponents of bf16 are those of fp32: the largest magnitude's top bits
 #pragma unroll
-        for (int u = 0; u < D / 8; ++u) {
-          const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = Pack2<T>::unpack(w[i]);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
+        for (int u = 0; u < kUnits; ++u) {
+          big = __vmaxu2(big, __vmaxu2(raw[u].x & 0x7fff7fffu, raw[u].y & 0x7fff7fffu));
+          big = __vmaxu2(big, __vmaxu2(raw[u].z & 0x7fff7fffu, raw[u].w & 0x7fff7fffu));
         }
-        const int e = max((__float_as_int(top) >> 23) - 127, -100);
+        const int mine = static_cast<int>(max(big & 0xffffu, big >> 16) >> 7) - 127;
+        const int e = max(max(mine, static_cast<int>(other(static_cast<float>(mine)))), -100);
         up = pow2(12 - e) * sign;
         down = pow2(e) * (scale / 4096.f);
       }
 #pragma unroll
-      for (int u = 0; u < D / 8; ++u) {
+      for (int u = 0; u < kUnits; ++u) {
         uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = Pack2<T>::unpack(w[i]);
           w[i] = pack_half(f.x * up, f.y * up);
         }
-        *reinterpret_cast<uint4 *>(smem + G::Q_OFF + (u / 8) * G::CHUNK_BYTES + unit_at(row, u % 8)) =
+        const int at = half * kUnits + u;
+        *reinterpret_cast<uint4 *>(smem + G::Q_OFF + (at / 8) * G::CHUNK_BYTES + unit_at(row, at % 8)) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
       fence_proxy_async_smem();
@@ -433,27 +463,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         ok = __all_sync(0xffffffffu, wait(&s_full[sb], (it >> 1) & 1, SITE_SFULL));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t s_tm = tmem_base + lane_off + sb * BN;
-        const int k0 = (sg.first + j) * BN;
-        uint32_t sr[BN];
-        tmem_ld4x32(s_tm, sr);
-        if (k0 + BN > keys) {
+        const uint32_t s_tm = tmem_base + lane_off + sb * BN, p_tm = tmem_base + lane_off + P_COL + sb * kHalf;
+        const int k0 = (sg.first + j) * BN, mine0 = k0 + half * kHalf;
+        // 32 scores at a time in registers; the first 32 are read again for their weights.
+        uint32_t sr[32];
+        auto scores = [&](int c) {
+          tmem_ld32(s_tm + half * kHalf + c, sr);
+          if (mine0 + c + 32 > keys) {
 #pragma unroll
-          for (int t = 0; t < BN; ++t)
-            if (k0 + t >= keys) sr[t] = __float_as_uint(-INFINITY);
+            for (int t = 0; t < 32; ++t)
+              if (mine0 + c + t >= keys) sr[t] = __float_as_uint(-INFINITY);
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) {
+          scores(c);
+          float mx4[4] = {mx, __uint_as_float(sr[0]), __uint_as_float(sr[1]), __uint_as_float(sr[2])};
+#pragma unroll
+          for (int t = 3; t < 31; t += 2)
+            mx4[(t >> 1) & 3] = max3f(mx4[(t >> 1) & 3], __uint_as_float(sr[t]), __uint_as_float(sr[t + 1]));
+          mx = max3f(max3f(mx4[0], mx4[1], mx4[2]), mx4[3], __uint_as_float(sr[31]));
         }
-        float mx8[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) mx8[t] = __uint_as_float(sr[t]);
-#pragma unroll
-        for (int t = 8; t < BN; t += 2)
-          mx8[(t >> 1) & 7] = max3f(mx8[(t >> 1) & 7], __uint_as_float(sr[t]), __uint_as_float(sr[t + 1]));
-        const float mx = rs * max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-        // O is stable once the previous tile's P V has completed.
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, wait(pv_done, (it - 1) & 1, SITE_PVDONE));
-          if (!ok) break;
-        }
+        mx = rs * fmaxf(mx, other(mx));
         float alpha = 1.0f;
         bool rescale = false;
         if (m_use == -INFINITY) {
@@ -466,37 +498,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         const float neg_m = m_use == -INFINITY ? 0.f : -m_use;
         // The exponents below are exact products less the rounded maximum, which is within half an ulp of
         // its own product; where half an ulp could be many units, round the products first.
-        float factor = rs;
-        if (__any_sync(0xffffffffu, fabsf(m_use) >= 268435456.f && m_use != -INFINITY)) {
-#pragma unroll
-          for (int t = 0; t < BN; ++t) sr[t] = __float_as_uint(__uint_as_float(sr[t]) * rs);
-          factor = 1.f;
-        }
+        const bool huge = __any_sync(0xffffffffu, fabsf(m_use) >= 268435456.f && m_use != -INFINITY);
+        const float factor = huge ? 1.f : rs;
         const uint64_t scale2 = f2_pack(factor, factor);
         const uint64_t negm2 = f2_pack(neg_m, neg_m);
-        uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+        uint64_t ps2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int hlf = 0; hlf < 2; ++hlf) {
-          uint32_t pk[32];
+        for (int c = kHalf - 32; c >= 0; c -= 32) {
+          if (c < kHalf - 32) scores(c);
+          if (huge) {
 #pragma unroll
-          for (int t = 0; t < 64; t += 2) {
-            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sr[64 * hlf + t]), __uint_as_float(sr[64 * hlf + t + 1])), scale2, negm2);
+            for (int t = 0; t < 32; ++t) sr[t] = __float_as_uint(__uint_as_float(sr[t]) * rs);
+          }
+          uint32_t pk[16];
+#pragma unroll
+          for (int t = 0; t < 32; t += 2) {
+            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sr[t]), __uint_as_float(sr[t + 1])), scale2, negm2);
             float x0, x1;
             f2_unpack(x2, x0, x1);
             const float p0 = ex2_approx(x0);
             const float p1 = ex2_approx(x1);
-            ps2[(t >> 1) & 3] = f2_add(ps2[(t >> 1) & 3], f2_pack(p0, p1));
+            ps2[(t >> 1) & 1] = f2_add(ps2[(t >> 1) & 1], f2_pack(p0, p1));
             pk[t >> 1] = pack_half(p0, p1);
           }
-          tmem_st32(s_tm + 32 * hlf, pk);
+          tmem_st16(p_tm + (half * kHalf + c) / 2, pk);
         }
-        float ps[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f2_unpack(ps2[i], ps[2 * i], ps[2 * i + 1]);
-        l_run = l_run * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
+        // The scores are read: their buffer may take the next but one tile's.
+        tc_fence_before();
+        mbar_arrive(smem_u32(&s_empty[sb]));
+        float ps[4];
+        f2_unpack(ps2[0], ps[0], ps[1]);
+        f2_unpack(ps2[1], ps[2], ps[3]);
+        l_run = l_run * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
         if (__any_sync(0xffffffffu, rescale)) {
+          // O is stable once the previous tile's P V has completed. (Only here, and at the segment's end,
+          // are these barriers waited for: two tiles earlier their P V had completed before S came.)
+          ok = __all_sync(0xffffffffu, wait(&pv_done[sb ^ 1], ((it - 1) >> 1) & 1, SITE_PVDONE));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t r[32];
             tmem_ld32(o_tm + c, r);
 #pragma unroll
@@ -507,8 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         // V's groups without numbers: the notes are overwritten only after this tile's P V.
         ok = __all_sync(0xffffffffu, wait(&v_full[sb], (it >> 1) & 1, SITE_VFULL));
         if (!ok) break;
-        if (*reinterpret_cast<const volatile uint64_t *>(smem + G::ANY_OFF + sb * kUnpackWarps) != 0)
-          for (int t = 0; t < BN && k0 + t < keys; ++t) bad |= smem[G::BAD_OFF + sb * BN + t];
+        if (*reinterpret_cast<const volatile uint64_t *>(smem + G::ANY_OFF + sb * kUnpackWarps) != 0) {
+#pragma unroll 1
+          for (int t = 0; t < BN && k0 + t < keys; ++t)
+            if (smem[G::ANY_OFF + sb * kUnpackWarps + t / kPieceTokens]) bad |= smem[G::BAD_OFF + sb * BN + t];
+        }
         tc_fence_before();
         mbar_arrive(smem_u32(p_full));
       }
@@ -516,12 +560,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
       // ---- the next segment's q goes in first: this one's products with Q are complete ----
       const Segment done = sg;
       const int64_t done_pos = pos;
-      const float done_m = m_use, done_l = l_run;
+      const float done_l = l_run + other(l_run);
       advance();
       if (more && tiles() > 0) rs = load_q();
-      // ---- results ----
+      // ---- results: this thread's half of the channels ----
       if (n > 0) {
-        ok = __all_sync(0xffffffffu, wait(pv_done, (it - 1) & 1, SITE_PVDONE));
+        ok = __all_sync(0xffffffffu, wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, SITE_PVDONE));
         if (!ok) break;
         tc_fence_after();
       }
@@ -531,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
       const float inv = 1.f / done_l;  // no key: 0 / 0
       T *o = static_cast<T *>(a.o) + (done.pl.row0 + rr / a.G) * a.so0 + (done.hk * a.G + rr % a.G) * a.so1;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         uint32_t r[32];
         if (n > 0) {
           tmem_ld32(o_tm + c, r);
@@ -567,8 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         tc_fence_before();
         mbar_arrive(smem_u32(o_free));
       }
-      if (!whole && in) a.ws_ml[slot] = make_float2(done_l == 0.f ? -INFINITY : (done_m == -INFINITY ? 0.f : done_m), done_l);
-      if (!whole && done.first == 0 && row == 0)
+      if (!whole && in && half == 0)
+        a.ws_ml[slot] = make_float2(done_l == 0.f ? -INFINITY : (m_use == -INFINITY ? 0.f : m_use), done_l);
+      if (!whole && done.first == 0 && threadIdx.x == 0)
         a.ws_open[worker] = Open{static_cast<int>((done_pos + done.nt - 1) / per) - worker + 1,
                                  2 * worker + (at_start ? 0 : 1), done.hk, done.pl.row0, done.pl.r0, done.pl.nr, 0, 0};
       at_start = false;
@@ -577,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == kUmmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);
   }
@@ -589,8 +634,6 @@ int launch(const Args &a, cudaStream_t st) {
   KernelLaunchInfo info;
   const int rc = prepare_kernel(reinterpret_cast<const void *>(kern), Geo<D>::SMEM_BYTES, kThreads, 1, &info);
   if (rc) return rc;
-  if (info.num_regs * kThreads < 128 * (kRegsRows + kRegsIssue + 2 * kRegsUnpack))
-    return fail(TLLM_ERR_CUDA, "paged kv4 prefill: built with %d registers per thread, the split needs more", info.num_regs);
   kern<<<a.workers, kThreads, Geo<D>::SMEM_BYTES, st>>>(a);
   return cuda_status(cudaGetLastError(), "paged kv4 prefill launch");
 }
