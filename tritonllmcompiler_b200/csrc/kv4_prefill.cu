@@ -92,11 +92,18 @@ struct Geo {
 
 constexpr uint32_t kSwizzle128 = 2;
 
+// Descriptors of a tile's k-steps differ from the first one's by a constant in the address field (the
+// issuing lane is on the critical path). Q, K: 16 channels of a row; V: 16 rows.
+__device__ __forceinline__ uint64_t kmajor_base(uint32_t base) { return make_sdesc(base, 16, 8 * 128, kSwizzle128); }
 template <int D>
-__device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int k) {
-  const int byte = k * 32;
-  return make_sdesc(base + (byte / 128) * Geo<D>::CHUNK_BYTES + (byte % 128), 16, 8 * 128, kSwizzle128);
+__device__ __forceinline__ constexpr uint64_t kmajor_step(int k) {
+  return static_cast<uint64_t>(((k / 4) * Geo<D>::CHUNK_BYTES + (k % 4) * 32) >> 4);
 }
+template <int D>
+__device__ __forceinline__ uint64_t vmajor_base(uint32_t base) {
+  return make_sdesc(base, Geo<D>::CHUNK_BYTES, 8 * 128, kSwizzle128);
+}
+constexpr uint64_t kVmajorStep = (16 * 128) >> 4;
 
 // Byte of 16-byte unit u (of 8 per 128-byte span) of a tile's row.
 __device__ __forceinline__ int unit_at(int row, int u) { return row * 128 + ((u ^ (row & 7)) << 4); }
@@ -136,12 +143,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
   uint64_t *v_full = bars + 5;     // [2]
   uint64_t *v_empty = bars + 7;    // [2]
   uint64_t *s_full = bars + 9;     // [2]
-  uint64_t *p_full = bars + 11;
-  uint64_t *pv_done = bars + 12;   // [2], as s_full by the tile's parity
-  uint64_t *o_free = bars + 14;
-  uint64_t *s_empty = bars + 15;   // [2]
-  uint64_t *pair = bars + 17;      // [4]
-  uint64_t *raw_full = bars + 21;                // [kRawStages]
+  // (Two, as of all barriers with a phase per tile: a phase must not pass unseen, and the next tile's
+  // weights can be complete before this tile's wait has looked.)
+  uint64_t *p_full = bars + 11;    // [2]
+  uint64_t *pv_done = bars + 13;   // [2], as s_full by the tile's parity
+  uint64_t *o_free = bars + 15;
+  uint64_t *s_empty = bars + 16;   // [2]
+  uint64_t *pair = bars + 18;      // [4]
+  uint64_t *raw_full = bars + 22;                // [kRawStages]
   uint64_t *raw_empty = raw_full + kRawStages;   // [kRawStages]
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(raw_empty + kRawStages);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
@@ -159,6 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
       mbar_init(smem_u32(&v_empty[s]), 1);
       mbar_init(smem_u32(&s_full[s]), 1);
       mbar_init(smem_u32(&s_empty[s]), kRowThreads);
+      mbar_init(smem_u32(&p_full[s]), kRowThreads);
       mbar_init(smem_u32(&pv_done[s]), 1);
     }
     for (int s = 0; s < kRawStages; ++s) {
@@ -166,7 +176,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
       mbar_init(smem_u32(&raw_empty[s]), kUnpackWarps);
     }
     for (int s = 0; s < 4; ++s) mbar_init(smem_u32(&pair[s]), 64);
-    mbar_init(smem_u32(p_full), kRowThreads);
     mbar_init(smem_u32(o_free), kRowThreads);
     *abort_flag = 0;
     fence_mbar_init();
@@ -356,10 +365,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         const int n = tiles();
         if (n == 0) continue;
         auto issue_qk = [&](uint32_t i) {
-          const uint32_t kbase = sK + (i & 1) * G::TILE_BYTES;
+          const uint64_t qd = kmajor_base(sQ), kd = kmajor_base(sK + (i & 1) * G::TILE_BYTES);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_f16_ss(tmem_base + (i & 1) * BN, kmajor_desc<D>(sQ, k), kmajor_desc<D>(kbase, k), idesc_qk,
+            umma_f16_ss(tmem_base + (i & 1) * BN, qd + kmajor_step<D>(k), kd + kmajor_step<D>(k), idesc_qk,
                         k != 0 ? 1u : 0u);
           umma_commit(smem_u32(&s_full[i & 1]));
           umma_commit(smem_u32(&k_empty[i & 1]));
@@ -374,15 +383,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         for (int j = 0; j < 2 && j < n && ok; ++j) next_qk(it + j);
         for (int j = 0; j < n && ok; ++j, ++it) {
           const uint32_t st = it & 1;
-          ok = wait(p_full, it & 1, SITE_PFULL) && wait(&v_full[st], (it >> 1) & 1, SITE_VFULL) &&
-               (j > 0 || seg == 0 || wait(o_free, (seg - 1) & 1, SITE_OFREE));
+          ok = (j > 0 || seg == 0 || wait(o_free, (seg - 1) & 1, SITE_OFREE)) &&
+               wait(&v_full[st], (it >> 1) & 1, SITE_VFULL) && wait(&p_full[st], (it >> 1) & 1, SITE_PFULL);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t vbase = sV + st * G::TILE_BYTES;
+          const uint64_t vd = vmajor_base<D>(sV + st * G::TILE_BYTES);
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            umma_f16_ts(tmem_base + O_COL, tmem_base + P_COL + st * kHalf + k * 8,
-                        make_sdesc(vbase + k * 16 * 128, G::CHUNK_BYTES, 8 * 128, kSwizzle128), idesc_pv,
+            umma_f16_ts(tmem_base + O_COL, tmem_base + P_COL + st * kHalf + k * 8, vd + k * kVmajorStep, idesc_pv,
                         (j | k) != 0 ? 1u : 0u);
           umma_commit(smem_u32(&v_empty[st]));
           umma_commit(smem_u32(&pv_done[st]));
@@ -476,6 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           }
         };
         float mx = -INFINITY;
+        ok = __all_sync(0xffffffffu, wait(&v_full[sb], (it >> 1) & 1, SITE_VFULL));  // (for the notes below)
+        if (!ok) break;
 #pragma unroll
         for (int c = 0; c < kHalf; c += 32) {
           scores(c);
@@ -546,15 +556,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           }
         }
         // V's groups without numbers: the notes are overwritten only after this tile's P V.
-        ok = __all_sync(0xffffffffu, wait(&v_full[sb], (it >> 1) & 1, SITE_VFULL));
-        if (!ok) break;
         if (*reinterpret_cast<const volatile uint64_t *>(smem + G::ANY_OFF + sb * kUnpackWarps) != 0) {
 #pragma unroll 1
           for (int t = 0; t < BN && k0 + t < keys; ++t)
             if (smem[G::ANY_OFF + sb * kUnpackWarps + t / kPieceTokens]) bad |= smem[G::BAD_OFF + sb * BN + t];
         }
         tc_fence_before();
-        mbar_arrive(smem_u32(p_full));
+        mbar_arrive(smem_u32(&p_full[sb]));
       }
       if (!ok) break;
       // ---- the next segment's q goes in first: this one's products with Q are complete ----
