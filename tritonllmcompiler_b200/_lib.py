@@ -231,6 +231,28 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(device: int, fn, *args) -> None:
+    """Calls a C entry point on ``device`` (an index) with its current stream as the last argument,
+    and raises for a non-zero status. Wrappers of calls that take a few microseconds on the GPU use
+    it: it touches nothing but the device index and the stream."""
+    if device == _get_device():
+        rc = fn(*args, _raw_stream(device) if _raw_stream is not None
+                else torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        check(rc)
+
+
+def int64s(*values: int):
+    """``values`` as a ctypes int64 array (strides kept with a checked set of shapes)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 def on_device(t: torch.Tensor):
     """Context making ``t``'s device current for the library call (the C entry points work on
     the current device); a no-op when it already is, which is the common case and saves the

@@ -10,6 +10,8 @@ exports, and they are imported from this module.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from tritonllmcompiler_b200 import _lib
@@ -26,22 +28,39 @@ def new_kv4_cache(num_blocks: int, num_kv_heads: int, block_size: int, head_dim:
                        dtype=torch.uint8, device=device)
 
 
-def _check_cache(cache: torch.Tensor, block_size: int) -> tuple[int, int, int]:
-    """(num_blocks, num_kv_heads, head_dim) of a cache made by ``new_kv4_cache`` (or a slice of a
-    larger one that keeps its two innermost dimensions together)."""
-    assert cache.is_cuda and cache.dim() == 4 and cache.dtype == torch.uint8
-    n, h, pieces, row = cache.shape
+@functools.lru_cache(maxsize=256)
+def _cache_sizes(shape: tuple, stride: tuple, dtype: torch.dtype, block_size: int):
+    """(num_blocks, num_kv_heads, head_dim, strides for the library) of a cache made by
+    ``new_kv4_cache``, or a slice of a larger one that keeps its two innermost dimensions together."""
+    assert len(shape) == 4 and dtype == torch.uint8
+    n, h, pieces, row = shape
     assert block_size in (16, 32, 64) and pieces == block_size // 16
     assert row in (1280, 2560), "head dim must be 64 or 128"
-    s = cache.stride()
-    assert s[3] == 1 and (s[2] == row or pieces == 1) and s[0] % 16 == 0 and s[1] % 16 == 0 \
-        and cache.data_ptr() % 16 == 0, "cache rows must be contiguous and 16-byte aligned"
-    return n, h, row // 20
+    assert stride[3] == 1 and (stride[2] == row or pieces == 1) and stride[0] % 16 == 0 and stride[1] % 16 == 0, \
+        "cache rows must be contiguous and 16-byte aligned"
+    return n, h, row // 20, _lib.int64s(*stride[:2])
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    s = t.stride()
-    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
+def _check_cache(cache: torch.Tensor, block_size: int):
+    assert cache.get_device() >= 0 and cache.data_ptr() % 16 == 0
+    return _cache_sizes(cache.shape, cache.stride(), cache.dtype, block_size)
+
+
+@functools.lru_cache(maxsize=256)
+def _row_strides(stride: tuple):
+    """The strides of [T, H, D] rows for the library, or None where it cannot read them."""
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8:
+        return None
+    return _lib.int64s(*stride[:2])
+
+
+def _rows(t: torch.Tensor):
+    """(the rows as the library reads them, their strides)."""
+    s = _row_strides(t.stride())
+    if s is None or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = _row_strides(t.stride())
+    return t, s
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:
@@ -54,38 +73,37 @@ def paged_kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slot
     place, for every t with slots[t] >= 0. A slot past the pool is skipped and flagged
     (``_lib.debug_status()`` returns 0x200). Groups that hold a NaN, an infinity or values beyond
     fp16's range do not read back as numbers."""
-    n, h, d = _check_cache(cache, block_size)
-    assert k.is_cuda and k.dim() == 3 and v.shape == k.shape and tuple(k.shape[1:]) == (h, d)
-    assert k.dtype in _lib.DTYPE_CODES and v.dtype == k.dtype
+    n, h, d, sc = _check_cache(cache, block_size)
     t = k.shape[0]
-    assert slots.shape == (t,)
-    assert k.device == cache.device and v.device == cache.device and slots.device == cache.device
+    assert k.shape == (t, h, d) and v.shape == k.shape and slots.shape == (t,)
+    assert k.dtype in _lib.DTYPE_CODES and v.dtype == k.dtype
+    device = cache.get_device()
+    assert k.get_device() == device and v.get_device() == device and slots.get_device() == device
     if t == 0:
         return
-    kk, vv = (x if _rows_ok(x) else x.contiguous() for x in (k, v))
+    k, sk = _rows(k)
+    v, sv = _rows(v)
     sl = _int32(slots)
-    with _lib.on_device(cache):
-        _lib.check(_lib.load().tllm_paged_kv4_append(
-            kk.data_ptr(), vv.data_ptr(), cache.data_ptr(), sl.data_ptr(), t, h, d, block_size, n,
-            _lib.strides(kk, 2), _lib.strides(vv, 2), _lib.strides(cache, 2),
-            _lib.DTYPE_CODES[k.dtype], _lib.stream_of(cache)))
+    _lib.launch(device, _lib.load().tllm_paged_kv4_append, k.data_ptr(), v.data_ptr(),
+                cache.data_ptr(), sl.data_ptr(), t, h, d, block_size, n, sk, sv, sc,
+                _lib.DTYPE_CODES[k.dtype])
 
 
 def paged_kv4_gather(cache: torch.Tensor, slots: torch.Tensor, *, block_size: int,
                      dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """The K and V rows ([T, Hkv, D] each, of the given dtype) that slots [T] hold; zeros where
     slots[t] < 0 or past the pool (the latter flagged)."""
-    n, h, d = _check_cache(cache, block_size)
-    assert dtype in _lib.DTYPE_CODES and slots.dim() == 1 and slots.device == cache.device
+    n, h, d, sc = _check_cache(cache, block_size)
+    device = cache.get_device()
+    assert dtype in _lib.DTYPE_CODES and slots.dim() == 1 and slots.get_device() == device
     t = slots.shape[0]
-    k = torch.empty((t, h, d), dtype=dtype, device=cache.device)
-    v = torch.empty((t, h, d), dtype=dtype, device=cache.device)
+    k = cache.new_empty((t, h, d), dtype=dtype)
+    v = torch.empty_like(k)
     sl = _int32(slots)
-    with _lib.on_device(cache):
-        _lib.check(_lib.load().tllm_paged_kv4_gather(
-            cache.data_ptr(), sl.data_ptr(), k.data_ptr(), v.data_ptr(), t, h, d, block_size, n,
-            _lib.strides(k, 2), _lib.strides(v, 2), _lib.strides(cache, 2),
-            _lib.DTYPE_CODES[dtype], _lib.stream_of(cache)))
+    so = _row_strides((h * d, d, 1))
+    _lib.launch(device, _lib.load().tllm_paged_kv4_gather, cache.data_ptr(), sl.data_ptr(),
+                k.data_ptr(), v.data_ptr(), t, h, d, block_size, n, so, so, sc,
+                _lib.DTYPE_CODES[dtype])
     return k, v
 
 
@@ -102,33 +120,31 @@ def paged_attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_tables: torc
     per sequence; prefill chunks, speculative tokens and idle sequences may be mixed in one call.
     Returns a new [T, Hq, D] tensor: NaN in rows that see no key, as in ``paged_attention``, and
     zeros in rows past cu_seqlens[B]."""
-    n, hkv, d = _check_cache(cache, block_size)
-    assert q.is_cuda and q.dim() == 3 and q.shape[2] == d and q.dtype in _lib.DTYPE_CODES
+    n, hkv, d, sc = _check_cache(cache, block_size)
+    assert q.dim() == 3 and q.shape[2] == d and q.dtype in _lib.DTYPE_CODES
     t, hq, _ = q.shape
     assert hkv >= 1 and hq % hkv == 0
     assert block_tables.dim() == 2 and context_lens.dim() == 1 and cu_seqlens.dim() == 1
-    b = block_tables.shape[0]
+    b, max_blocks = block_tables.shape
     assert context_lens.shape[0] == b and cu_seqlens.shape[0] == b + 1
-    assert q.device == cache.device and block_tables.device == cache.device
-    assert context_lens.device == cache.device and cu_seqlens.device == cache.device
+    device = cache.get_device()
+    assert q.get_device() == device and block_tables.get_device() == device
+    assert context_lens.get_device() == device and cu_seqlens.get_device() == device
     if sm_scale is None:
         sm_scale = d ** -0.5
-    out = torch.empty((t, hq, d), device=q.device, dtype=q.dtype)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if t == 0 or hq == 0:
         return out
-    qq = q if _rows_ok(q) else q.contiguous()
+    q, sq = _rows(q)
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
     cl, cu = _int32(context_lens), _int32(cu_seqlens)
     max_new = min(int(max_new), t)
     lib = _lib.load()
-    with _lib.on_device(q):
-        ws_bytes = lib.tllm_paged_kv4_attn_workspace_size(b, t, hq, hkv, max_new, d, block_size,
-                                                          bt.shape[1])
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        _lib.check(lib.tllm_paged_kv4_attn(
-            qq.data_ptr(), cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), cu.data_ptr(),
-            out.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, b, t, hq, hkv,
-            max_new, d, block_size, bt.shape[1], n, _lib.strides(qq, 2), _lib.strides(cache, 2),
-            _lib.strides(bt), _lib.strides(out, 2), float(sm_scale), int(bool(causal)),
-            _lib.DTYPE_CODES[q.dtype], _lib.stream_of(q)))
+    ws_bytes = lib.tllm_paged_kv4_attn_workspace_size(b, t, hq, hkv, max_new, d, block_size, max_blocks)
+    ws = cache.new_empty((ws_bytes,))
+    _lib.launch(device, lib.tllm_paged_kv4_attn, q.data_ptr(), cache.data_ptr(), bt.data_ptr(),
+                cl.data_ptr(), cu.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes, b, t, hq,
+                hkv, max_new, d, block_size, max_blocks, n, sq, sc, _lib.strides(bt),
+                _row_strides((hq * d, d, 1)), float(sm_scale), int(bool(causal)),
+                _lib.DTYPE_CODES[q.dtype])
     return out

@@ -36,22 +36,19 @@ def paged_plan(block_tables: torch.Tensor, seq_lens: torch.Tensor, n_new: torch.
     (at least the sum of n_new; rows past that sum get slot -1 and position 0). A sequence that
     its table row, the free list or max_tokens cannot hold is refused whole: its slots are -1,
     its new length is the old one and its table row stays. Negative lengths count as 0."""
-    assert block_tables.is_cuda and block_tables.dim() == 2 and block_tables.dtype == torch.int32
+    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32
+    device = block_tables.get_device()
     b, max_blocks = block_tables.shape
-    assert seq_lens.shape == (b,) and n_new.shape == (b,) and free_blocks.dim() == 1
-    dev = block_tables.device
-    assert seq_lens.device == dev and n_new.device == dev and free_blocks.device == dev
+    assert device >= 0 and seq_lens.shape == (b,) and n_new.shape == (b,) and free_blocks.dim() == 1
+    assert seq_lens.get_device() == device and n_new.get_device() == device
+    assert free_blocks.get_device() == device and block_size >= 1 and max_tokens >= 0
     max_tokens = int(max_tokens)
-    assert block_size >= 1 and max_tokens >= 0
     sl, nn, fb = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
                   for t in (seq_lens, n_new, free_blocks))
-    out = torch.empty(2 * max_tokens + 2 * b + 2, dtype=torch.int32, device=dev)
-    plan = PagedPlan(*out.split_with_sizes((max_tokens, max_tokens, b + 1, b, 1)))
+    out = block_tables.new_empty((2 * max_tokens + 2 * b + 2,))
     at = out.data_ptr()
-    with _lib.on_device(block_tables):
-        _lib.check(_lib.load().tllm_paged_plan(
-            block_tables.data_ptr(), sl.data_ptr(), nn.data_ptr(), fb.data_ptr(), at,
-            at + 4 * max_tokens, at + 8 * max_tokens, at + 4 * (2 * max_tokens + b + 1),
-            at + 4 * (2 * max_tokens + 2 * b + 1), b, max_blocks, fb.shape[0], max_tokens,
-            block_size, _lib.strides(block_tables), _lib.stream_of(block_tables)))
-    return plan
+    _lib.launch(device, _lib.load().tllm_paged_plan, block_tables.data_ptr(), sl.data_ptr(),
+                nn.data_ptr(), fb.data_ptr(), at, at + 4 * max_tokens, at + 8 * max_tokens,
+                at + 4 * (2 * max_tokens + b + 1), at + 4 * (2 * max_tokens + 2 * b + 1), b,
+                max_blocks, fb.shape[0], max_tokens, block_size, _lib.strides(block_tables))
+    return PagedPlan(*out.split_with_sizes((max_tokens, max_tokens, b + 1, b, 1)))

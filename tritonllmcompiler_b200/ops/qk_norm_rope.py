@@ -22,11 +22,6 @@ import torch
 from tritonllmcompiler_b200 import _lib
 
 
-def _ok(t: torch.Tensor) -> bool:
-    s = t.stride()
-    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
-
-
 @functools.lru_cache(maxsize=64)
 def _axis_words(sections: tuple, interleaved: bool, half: int):
     """The axis of each rotary pair, 2 bits each, as the library takes them."""
@@ -45,31 +40,76 @@ def _axis_words(sections: tuple, interleaved: bool, half: int):
     return words
 
 
-def _arguments(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved):
-    """Checks shared by both directions; the tensors as the library takes them."""
-    assert q.is_cuda and q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0]
-    t, _, d = q.shape
-    assert d in (16, 32, 64, 128) and k.shape[2] == d
-    assert q.dtype in _lib.DTYPE_CODES and k.dtype == q.dtype
-    assert q_weight.shape == (d,) and k_weight.shape == (d,)
-    assert q_weight.dtype == q.dtype and k_weight.dtype == q.dtype
-    assert cos.dim() == 2 and cos.shape[1] == d // 2 and sin.shape == cos.shape
-    assert cos.dtype == torch.float32 and sin.dtype == torch.float32
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    assert positions.dim() == 2 and positions.shape[1] == t
-    sections = (d // 2,) if sections is None else tuple(sections)
-    assert positions.shape[0] == len(sections), "one row of positions per section"
-    for x in (k, q_weight, k_weight, cos, sin, positions):
-        assert x.device == q.device
-    words = _axis_words(sections, bool(interleaved), d // 2)
-    if positions.dtype != torch.int32 or positions.stride(1) != 1:
-        positions = positions.to(torch.int32).contiguous()
-    q, k = (x if _ok(x) else x.contiguous() for x in (q, k))
-    vec = lambda x, m: x.stride(-1) == 1 and x.stride(0) % m == 0 and x.data_ptr() % 16 == 0  # noqa: E731
-    cos, sin = (x if vec(x, 4) else x.contiguous() for x in (cos, sin))
-    q_weight, k_weight = (x if vec(x, 1) else x.contiguous().clone() for x in (q_weight, k_weight))
-    return q, k, q_weight, k_weight, cos, sin, positions, words
+def _rows_ok(stride: tuple) -> bool:
+    return stride[2] == 1 and stride[0] % 8 == 0 and stride[1] % 8 == 0
+
+
+def _table_ok(stride: tuple) -> bool:
+    return stride[1] == 1 and stride[0] % 4 == 0
+
+
+@functools.lru_cache(maxsize=256)
+def _checked(q, sq, k, sk, wq, swq, wk, swk, cos, scos, sin, ssin, pos, spos, dtypes, sections, interleaved,
+             *grads):
+    """Checks a set of shapes, strides and types, once (a call's checks took longer than the kernel at
+    one decode step). Returns what the library takes of them, or None where something has to be
+    copied first."""
+    assert len(q) == 3 and len(k) == 3 and k[0] == q[0]
+    t, _, d = q
+    assert d in (16, 32, 64, 128) and k[2] == d
+    dtype, k_dtype, wq_dtype, wk_dtype, cos_dtype, sin_dtype, pos_dtype = dtypes[:7]
+    assert dtype in _lib.DTYPE_CODES and k_dtype == dtype
+    assert wq == (d,) and wk == (d,) and wq_dtype == dtype and wk_dtype == dtype
+    assert len(cos) == 2 and cos[1] == d // 2 and sin == cos
+    assert cos_dtype == torch.float32 and sin_dtype == torch.float32
+    axes = 1 if len(pos) == 1 else pos[0]
+    assert len(pos) in (1, 2) and pos[-1] == t
+    sections = (d // 2,) if sections is None else sections
+    assert axes == len(sections), "one row of positions per section"
+    words = _axis_words(sections, interleaved, d // 2)
+    if grads:
+        assert grads[0] == q and grads[2] == k and dtypes[7] == dtype and dtypes[8] == dtype
+    ready = all(_rows_ok(x) for x in (sq, sk, *grads[1::2])) and swq == (1,) and swk == (1,)
+    ready = ready and _table_ok(scos) and _table_ok(ssin) and pos_dtype == torch.int32 and spos[-1] == 1
+    if not ready:
+        return None
+    table = (cos[0], scos[0], ssin[0], axes, spos[0] if len(pos) == 2 else t, words)
+    return (t, q[1], k[1], d), table, [_lib.int64s(*s[:2]) for s in (*grads[1::2], sq, sk)], \
+        [_lib.int64s(x[1] * d, d) for x in (q, k)], _lib.DTYPE_CODES[dtype]
+
+
+def _arguments(tensors, sections, interleaved):
+    """(tensors as the library takes them, what _checked gives): q, k, weights, cos, sin, positions and,
+    for the backward pass, the gradients of the two outputs."""
+    q, k, wq, wk, cos, sin, pos = tensors[:7]
+    if sections is not None and type(sections) is not tuple:
+        sections = tuple(sections)
+    device = q.get_device()
+    assert device >= 0 and all([x.get_device() == device for x in tensors])
+    address = q.data_ptr() | k.data_ptr() | wq.data_ptr() | wk.data_ptr() | cos.data_ptr() | sin.data_ptr()
+    more = ()
+    if len(tensors) > 7:
+        dqo, dko = tensors[7:]
+        address |= dqo.data_ptr() | dko.data_ptr()
+        more = (dqo.shape, dqo.stride(), dko.shape, dko.stride())
+    known = _checked(q.shape, q.stride(), k.shape, k.stride(), wq.shape, wq.stride(), wk.shape,
+                     wk.stride(), cos.shape, cos.stride(), sin.shape, sin.stride(), pos.shape,
+                     pos.stride(), tuple([x.dtype for x in tensors]), sections, bool(interleaved), *more)
+    if known is None or address % 16:
+        return _arguments(_readable(tensors), sections, interleaved)
+    return tensors, known, device
+
+
+def _readable(tensors):
+    """The tensors with those that the library cannot read where they are copied."""
+    def fix(i, x):
+        s = x.stride()
+        if i == 6:
+            return x.to(torch.int32) if s[-1] == 1 else x.to(torch.int32).clone(memory_format=torch.contiguous_format)
+        ok = s == (1,) if i in (2, 3) else _table_ok(s) if i in (4, 5) else _rows_ok(s)
+        return x if ok and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+    return tuple([fix(i, x) for i, x in enumerate(tensors)])
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -83,19 +123,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     positions: [T], or [axes, T] with one row per entry of sections (rotary pairs per axis, adding
     up to D / 2; one axis by default). interleaved=False gives the axes consecutive sections;
     interleaved=True gives axis a > 0 the pairs a, a + axes, a + 2 axes, ..., as many as its section
-    says while the pairs last, and the first axis all others. A position outside the table uses row 0 and is flagged
-    (``_lib.debug_status()`` returns 0x200). Returns new contiguous tensors."""
-    q, k, wq, wk, cos, sin, pos, words = _arguments(q, k, q_weight, k_weight, cos, sin, positions,
-                                                    sections, interleaved)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with _lib.on_device(q):
-        _lib.check(_lib.load().tllm_qk_norm_rope(
-            q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(),
-            sin.data_ptr(), pos.data_ptr(), qo.data_ptr(), ko.data_ptr(), q.shape[0], q.shape[1],
-            k.shape[1], q.shape[2], cos.shape[0], cos.stride(0), sin.stride(0), pos.shape[0],
-            pos.stride(0), words, _lib.strides(q, 2), _lib.strides(k, 2), _lib.strides(qo, 2),
-            _lib.strides(ko, 2), eps, _lib.DTYPE_CODES[q.dtype], _lib.stream_of(q)))
+    says while the pairs last, and the first axis all others. A position outside the table uses
+    row 0 and is flagged (``_lib.debug_status()`` returns 0x200). Returns new contiguous tensors."""
+    (q, k, wq, wk, cos, sin, pos), (sizes, table, strides, out_strides, code), device = _arguments(
+        (q, k, q_weight, k_weight, cos, sin, positions), sections, interleaved)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+    _lib.launch(device, _lib.load().tllm_qk_norm_rope, q.data_ptr(), k.data_ptr(), wq.data_ptr(),
+                wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), qo.data_ptr(),
+                ko.data_ptr(), *sizes, *table, *strides, *out_strides, eps, code)
     return qo, ko
 
 
@@ -107,30 +143,19 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     """(dq, dk, dq_weight, dk_weight) of ``qk_norm_rope`` at its inputs, given the gradients of
     its two outputs. The norms are recomputed from q and k; the weights' gradients are summed in
     fp32 in a fixed order, so equal inputs give equal bits."""
-    assert dq_out.shape == q.shape and dk_out.shape == k.shape
-    assert dq_out.dtype == q.dtype and dk_out.dtype == q.dtype
-    assert dq_out.device == q.device and dk_out.device == q.device
-    q, k, wq, wk, cos, sin, pos, words = _arguments(q, k, q_weight, k_weight, cos, sin, positions,
-                                                    sections, interleaved)
-    dqo, dko = (x if _ok(x) else x.contiguous() for x in (dq_out, dk_out))
-    t, hq, d = q.shape
-    hkv = k.shape[1]
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    dw = torch.empty((2, d), dtype=q.dtype, device=q.device)
+    (q, k, wq, wk, cos, sin, pos, dqo, dko), (sizes, table, strides, out_strides, code), device = _arguments(
+        (q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out), sections, interleaved)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
     lib = _lib.load()
-    with _lib.on_device(q):
-        ws_bytes = lib.tllm_qk_norm_rope_bwd_workspace_size(t, hq, hkv, d)
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-        _lib.check(lib.tllm_qk_norm_rope_bwd(
-            dqo.data_ptr(), dko.data_ptr(), q.data_ptr(), k.data_ptr(), wq.data_ptr(),
-            wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dw.data_ptr(), dw.data_ptr() + d * dw.element_size(), ws.data_ptr(),
-            ws_bytes, t, hq, hkv, d, cos.shape[0], cos.stride(0), sin.stride(0), pos.shape[0],
-            pos.stride(0), words, _lib.strides(dqo, 2), _lib.strides(dko, 2), _lib.strides(q, 2),
-            _lib.strides(k, 2), _lib.strides(dq, 2), _lib.strides(dk, 2), eps,
-            _lib.DTYPE_CODES[q.dtype], _lib.stream_of(q)))
-    return dq, dk, dw[0], dw[1]
+    ws_bytes = lib.tllm_qk_norm_rope_bwd_workspace_size(*sizes)
+    ws = cos.new_empty((ws_bytes // 4 + 4,))
+    _lib.launch(device, lib.tllm_qk_norm_rope_bwd, dqo.data_ptr(), dko.data_ptr(), q.data_ptr(),
+                k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                pos.data_ptr(), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+                ws.data_ptr(), ws_bytes, *sizes, *table, *strides, *out_strides, eps, code)
+    return dq, dk, dwq, dwk
 
 
 class _QkNormRope(torch.autograd.Function):
