@@ -294,13 +294,15 @@ int forward_d(const Args &a, cudaStream_t st) {
   return cuda_status(cudaGetLastError(), "qk_norm_rope launch");
 }
 
-// Blocks of the backward pass: two per SM at most, shared between queries and keys by their rows.
+// Blocks of the backward pass: eight per SM at most (four waves; with the two that fit at once, and no
+// new ones to start while others end, 8192 tokens took 79 us instead of 65), shared between queries
+// and keys by their rows.
 void plan_blocks(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int (&blocks)[2]) {
   const int64_t sms = sm_count() > 0 ? sm_count() : 148;
   const int64_t rows[2] = {T * Hq, T * Hkv}, all = rows[0] + rows[1];
   const int64_t groups = kThreads / (D / 16);  // rows a block takes at once
   for (int i = 0; i < 2; ++i) {
-    const int64_t share = (2 * sms * rows[i] + all - 1) / std::max<int64_t>(all, 1);
+    const int64_t share = (8 * sms * rows[i] + all - 1) / std::max<int64_t>(all, 1);
     blocks[i] = static_cast<int>(std::min(share, (rows[i] + groups - 1) / groups));
   }
 }
