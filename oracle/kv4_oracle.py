@@ -96,7 +96,7 @@ def quantise(x):
         sf, zf = np.float32(s), np.float32(z)
         inv = np.where(sf > 0, np.float32(1) / sf, np.float32(0))
         codes = np.clip(np.rint((g - zf) * inv), 0, 15)
-    return codes, np.float64(s), np.float64(z)
+    return codes, s.astype(np.float64), z.astype(np.float64)
 
 
 def dequantise(codes, s, z):

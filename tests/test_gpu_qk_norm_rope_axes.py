@@ -82,27 +82,6 @@ def test_backward(cuda_device, T, hq, hkv, D, sections, mix, dtype):
     assert _lib.debug_status() == 0
 
 
-def test_gradient_against_differences(cuda_device):
-    """The oracle's gradient against central differences of its forward, in 64 bits: the step's
-    error is of the order of 1e-5 squared times third derivatives, the cancellation's 1e-16 / 1e-5."""
-    rng = np.random.RandomState(3)
-    T, H, D, sec = 2, 2, 16, (3, 5)
-    x, dz = rng.randn(T, H, D), rng.randn(T, H, D)
-    w, ang = 1 + 0.2 * rng.randn(D), rng.randn(11, 8)
-    pos = rng.randint(0, 11, (2, T))
-    f = lambda x, w: (O.norm_rope(x, w, np.cos(ang), np.sin(ang), pos, sec) * dz).sum()  # noqa: E731
-    dx, dw, _, _ = O.norm_rope_grad(dz, x, w, np.cos(ang), np.sin(ang), pos, sec)
-    e = 1e-5
-    for i in np.ndindex(x.shape):
-        d = np.zeros_like(x)
-        d[i] = e
-        assert abs((f(x + d, w) - f(x - d, w)) / (2 * e) - dx[i]) < 1e-7
-    for i in range(D):
-        d = np.zeros_like(w)
-        d[i] = e
-        assert abs((f(x, w + d) - f(x, w - d)) / (2 * e) - dw[i]) < 1e-7
-
-
 def test_autograd(cuda_device):
     q, k, wq, wk, cos, sin, pos = _case(9, 33, 4, 2, 64, (32,), torch.bfloat16)
     leaves = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
