@@ -38,6 +38,10 @@ constexpr int kMergeLoads = 8;  // parts a merging warp reads at a time
 constexpr int kMinTiles = 2;  // a warp's least run of tiles
 constexpr int kSplitRows = 32;  // query rows per sequence and KV head up to which kv4_split_kernel runs
 
+// CTAs of the split kernel per SM: what its registers allow without spilling much (two row tiles of 8 in
+// 168 registers, three CTAs, took 175 us where 157 do; one in 128, four CTAs, 135 where 123 did).
+__host__ __device__ constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
+
 enum : int { SITE_TILE = 0x41 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -95,18 +99,21 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 //           exact in fp16 from either type, so scores are exact but for fp32 sums.
 //   o_d   = sum_t (p_t s_{t,g}) (c_{t,d} - 8) + sum_t p_t (z_{t,g} + 8 s_{t,g}): weights are fp16, and
 //           fp16 again after the scale (packed products on the transposed weights, a third of the
-//           instructions of fp32 ones), so their rounding errors meet values centred on 0 in
-//           both sums: without the 8 they would meet values of twice that size that cancel. The 8 is
-//           one MMA with a constant operand for each of the codes'. The second sum is an MMA.
+//           instructions of fp32 ones). The second sum is one more MMA. The 8 centres both sums on
+//           0: without it two sums of twice the size cancel, with 2.4 times the rounding errors, and over
+//           100,000 keys the MMAs' truncating sums alone doubled the error of a bf16 output. For fp16
+//           outputs the low parts that the rounding after the scale leaves out are multiplied too
+//           (error 1.4 times that of rounding the output, against 1.6, for 5 % of the time).
 // Weights are 2^(x - mu) with mu = m - k: k <= 12 keeps the weights times the scales in fp16's normal
 // range whatever the size of V (from the largest scale met), and m follows the maximum only
 // when it grows by more than 2^3 (weights and products stay under 2^15).
 // An S^T result becomes a P^T operand by transposing 8 x 8 blocks in registers (movmatrix).
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const Args a) {
   using P = Piece<D>;
   constexpr int W = P::W;
   constexpr int ROWS = 8 * NT;
+  constexpr bool kLow = std::is_same<T, __half>::value;  // weights times scales with their low parts
   constexpr int TILE_BYTES = 2 * P::BYTES;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[kWarps][kStages];
@@ -436,6 +443,16 @@ __global__ void __launch_bounds__(kThreads, 3) kv4_split_kernel(const Args a) {
           }
           mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], w0, w1);
           mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], w0, w1);
+          if constexpr (kLow) {  // what the products' rounding left out, exactly
+            uint32_t r0 = fma_half2(b0[j], s0[g], w0 ^ 0x80008000u);
+            uint32_t r1 = fma_half2(b1[j], s1[g], w1 ^ 0x80008000u);
+            if constexpr (kMask) {
+              r0 &= ~zero_halves(b0[j]);
+              r1 &= ~zero_halves(b1[j]);
+            }
+            mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], r0, r1);
+            mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], r0, r1);
+          }
         }
       }
     }
@@ -585,7 +602,7 @@ Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t D, i
   const int64_t sms = sm_count() > 0 ? sm_count() : 148;
   const int64_t most = B * p.n_rt * Hkv * std::max<int64_t>((max_blocks * block_size + tile - 1) / tile, 1);
   const int64_t each = p.nt > 0 ? kWarps * kMinTiles : 1;  // a CTA's least run
-  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(p.nt > 0 ? 3 * sms : sms, (most + each - 1) / each)));
+  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(p.nt > 0 ? resident(p.nt) * sms : sms, (most + each - 1) / each)));
   p.workers = p.ctas * (p.nt > 0 ? kWarps : 1);
   const size_t workers = static_cast<size_t>(p.workers), rows_all = 2 * workers * row_tile;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
