@@ -8,11 +8,16 @@
 // exact ones would, a fraction of the half step of 1 / 30, for 4 bytes per 16 bytes of codes. A
 // group with a NaN or an infinity, or beyond fp16's range, reads back as NaN or infinities.
 //
-// Bound: HBM, 2 bytes in and 0.625 out per element (the other way round when reading back). D / 8
-// consecutive lanes hold a row of K and the same row of V, one 16-byte vector of each; minimum and
-// maximum take two shuffles within the four lanes of a group. A lane's V codes belong to two
-// chunks of the layout, so pairs of lanes exchange halves and each lane stores one whole word.
-// No two lanes write the same byte, so tokens of one piece may be appended in any order.
+// Bound: HBM, 2 bytes in and 0.625 out per element (the other way round when reading back), if the
+// arithmetic stays at a few instructions per element. So a lane that writes holds a whole group of
+// K or of V (64 bytes): minimum and maximum are packed 16-bit operations without shuffles, there is
+// one reciprocal per group, differences and products are fp32 pairs, rounding and conversion are one
+// addition, and a group whose ends round into 0 .. 15 needs no clamps inside. 16001 tokens of 8
+// heads of 128: 27 us, 3 TB/s (a lane per 8 channels of both, each clamped and converted: 32 us). The
+// lanes' 64 registers leave 32 warps an SM, and what one token writes is 8 to 16 bytes at a time,
+// so latency and partial sectors hold it now, not issue. Reading back needs no group in one lane: 8
+// channels of K and V each make wide coalesced stores, 20 us and 4 TB/s for the same rows (a group per
+// lane: 28). No two lanes write the same byte, so tokens of one piece may be appended in any order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -55,52 +60,81 @@ struct Args {
   int64_t num_slots;
 };
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+// Packed minimum and maximum that keep NaNs.
+__device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2_nan(a, b); }
+__device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
+template <typename T>
+struct Two;
+template <>
+struct Two<__half> {
+  using type = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
-// The codes of the lane's 8 channels (channel i at bits 4 i) and its group's scale and zero. All
-// four lanes of the group take part.
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half &s, __half &z) {
-  float lo = x[0], hi = x[0];
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23: y + kRound has y, rounded to even, in its low bits
+// Sum of 16^i times the bits of kRound over four codes: what Horner's rule over the raw sums adds.
+constexpr uint32_t kRoundBits = 0x4b400000u;
+constexpr uint32_t kRoundFour = kRoundBits * 0x1111u;
+
+// A group's 32 channels, two a word: its scale and zero, and sums[i] = kRoundBits + code i.
+template <typename T>
+__device__ __forceinline__ void quantise(const uint32_t (&w)[16], __half &s, __half &z, uint32_t (&sums)[32]) {
+  using T2 = typename Two<T>::type;
+  T2 lo2 = *reinterpret_cast<const T2 *>(&w[0]), hi2 = lo2;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
+  for (int i = 1; i < 16; ++i) {
+    const T2 v = *reinterpret_cast<const T2 *>(&w[i]);
+    lo2 = min2(lo2, v);
+    hi2 = max2(hi2, v);
   }
-#pragma unroll
-  for (int off = 1; off <= 2; off <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-  }
+  const float2 l = Pack2<T>::unpack(*reinterpret_cast<const uint32_t *>(&lo2));
+  const float2 h = Pack2<T>::unpack(*reinterpret_cast<const uint32_t *>(&hi2));
+  // A NaN in either half has to stay.
+  const float lo = l.x <= l.y ? l.x : (l.y < l.x ? l.y : __fadd_rn(l.x, l.y));
+  const float hi = h.x >= h.y ? h.x : (h.y > h.x ? h.y : __fadd_rn(h.x, h.y));
   s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   z = __float2half_rn(lo);
   const float sf = __half2float(s), zf = __half2float(z);
   const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
-  uint32_t codes = 0;
+  // All steps are monotonic: if the ends stay inside, so does everything between.
+  const bool inside = __fmul_rn(__fsub_rn(lo, zf), inv) >= -0.5f && __fmul_rn(__fsub_rn(hi, zf), inv) < 15.5f;
+  const uint64_t mz = f2_pack(-zf, -zf), inv2 = f2_pack(inv, inv);
+  if (inside) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], zf), inv)), 0.f), 15.f);  // NaN: 0
-    codes |= static_cast<uint32_t>(c) << (4 * i);
+    for (int i = 0; i < 16; ++i) {
+      const float2 f = Pack2<T>::unpack(w[i]);
+      float a, b;
+      f2_unpack(f2_mul(f2_add(f2_pack(f.x, f.y), mz), inv2), a, b);
+      sums[2 * i] = __float_as_uint(__fadd_rn(a, kRound));  // (a packed sum is contracted with the product)
+      sums[2 * i + 1] = __float_as_uint(__fadd_rn(b, kRound));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 f = Pack2<T>::unpack(w[i]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float y = __fmul_rn(__fsub_rn(e ? f.y : f.x, zf), inv);
+        sums[2 * i + e] = __float_as_uint(__fadd_rn(fminf(fmaxf(y, 0.f), 15.f), kRound));  // NaN: 0
+      }
+    }
   }
-  return codes;
 }
 
-// Channels j at bits 4 j -> bits 4 (j / 2) + 16 (j % 2).
-__device__ __forceinline__ uint32_t split_parity(uint32_t c) {
-  uint32_t even = c & 0x0f0f0f0fu, odd = (c >> 4) & 0x0f0f0f0fu;
-  even = (even | (even >> 4)) & 0x00ff00ffu;
-  odd = (odd | (odd >> 4)) & 0x00ff00ffu;
-  even = (even | (even >> 8)) & 0xffffu;
-  odd = (odd | (odd >> 8)) & 0xffffu;
-  return even | (odd << 16);
+// Four codes at bits 0, 4, 8, 12.
+__device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return ((d * 16u + c) * 16u + b) * 16u + a - kRoundFour;
 }
 
 __device__ __forceinline__ uint8_t *piece_of(const Args &a, int64_t slot, int h, int bytes) {
@@ -108,50 +142,67 @@ __device__ __forceinline__ uint8_t *piece_of(const Args &a, int64_t slot, int h,
   return a.cache + (slot >> a.log2_bs) * a.sblk + h * a.shead + (in / kPieceTokens) * bytes;
 }
 
+// 2 W lanes a row: the W groups of K, then those of V.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const Args a, uint32_t rows) {
   using P = Piece<D>;
-  constexpr int LANES = D / 8;
-  const uint32_t raw = (blockIdx.x * kThreads + threadIdx.x) / LANES;
-  bool ok = raw < rows;  // lanes past the end recompute the last row (for the shuffles)
-  const uint32_t row = ok ? raw : rows - 1;
+  constexpr int LANES = 2 * P::W;
+  const uint32_t row = (blockIdx.x * kThreads + threadIdx.x) / LANES;
+  if (row >= rows) return;
   const uint32_t t = row / a.H;
   const int h = row % a.H;
-  const int x = threadIdx.x % LANES;
+  const int g = threadIdx.x % P::W;
+  const bool is_v = (threadIdx.x % LANES) >= P::W;
   const int64_t slot = __ldg(a.slots + t);
-  const T *kp = static_cast<const T *>(a.k) + static_cast<int64_t>(t) * a.skt + h * a.skh + 8 * x;
-  const T *vp = static_cast<const T *>(a.v) + static_cast<int64_t>(t) * a.svt + h * a.svh + 8 * x;
-  const uint4 kr = ld_stream(kp), vr = ld_stream(vp);
-  if (slot >= a.num_slots && ok) atomicCAS(&g_kv4_status, 0, TLLM_DEV_BAD_INDEX);
-  ok = ok && slot >= 0 && slot < a.num_slots;
-  float kf[8], vf[8];
-  unpack8<T>(kr, kf);
-  unpack8<T>(vr, vf);
-  __half ks, kz, vs, vz;
-  const uint32_t kc = split_parity(quantise(kf, ks, kz));
-  const uint32_t vc = quantise(vf, vs, vz);
-  // Lane x = 4 g + m has V channels 32 g + 8 m + {0..7}: chunks n = 2 m (low half) and 2 m + 1. It
-  // stores chunk n = x / (W / 2), groups 2 y and 2 y + 1 with y = x % (W / 2).
-  constexpr int Y = P::W / 2;
-  const int n = x / Y, y = x % Y;
-  const int base = threadIdx.x & 31 & ~(LANES - 1);
-  const uint32_t g0 = __shfl_sync(0xffffffffu, vc, base + 8 * y + (n >> 1));
-  const uint32_t g1 = __shfl_sync(0xffffffffu, vc, base + 8 * y + 4 + (n >> 1));
-  const uint32_t vw = __byte_perm(g0, g1, (n & 1) ? 0x7632 : 0x5410);
-  if (!ok) return;
+  const T *src = is_v ? static_cast<const T *>(a.v) + static_cast<int64_t>(t) * a.svt + h * a.svh
+                      : static_cast<const T *>(a.k) + static_cast<int64_t>(t) * a.skt + h * a.skh;
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + kGroup * g + 8 * i));  // a line is read in four goes: keep it
+    w[4 * i] = v.x;
+    w[4 * i + 1] = v.y;
+    w[4 * i + 2] = v.z;
+    w[4 * i + 3] = v.w;
+  }
+  if (slot >= a.num_slots) atomicCAS(&g_kv4_status, 0, TLLM_DEV_BAD_INDEX);
+  if (slot < 0 || slot >= a.num_slots) return;
+  __half s, z;
+  uint32_t c[32];
+  quantise<T>(w, s, z, c);
   uint8_t *p = piece_of(a, slot, h, P::BYTES);
   const int tok = static_cast<int>(slot & (kPieceTokens - 1));
-  *reinterpret_cast<uint32_t *>(p + P::k_word(tok, x)) = kc;
-  *reinterpret_cast<uint32_t *>(p + P::v_bits(tok, 2 * y, n)) = vw;
-  const int g = x >> 2;
-  switch (x & 3) {
-    case 0: *reinterpret_cast<__half *>(p + P::k_scale(tok, g)) = ks; break;
-    case 1: *reinterpret_cast<__half *>(p + P::k_zero(tok, g)) = kz; break;
-    case 2: *reinterpret_cast<__half *>(p + P::v_scale(tok, g)) = vs; break;
-    default: *reinterpret_cast<__half *>(p + P::v_zero(tok, g)) = vz; break;
+  if (is_v) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+      *reinterpret_cast<uint16_t *>(p + P::v_bits(tok, g, n)) =
+          static_cast<uint16_t>(four(c[4 * n], c[4 * n + 1], c[4 * n + 2], c[4 * n + 3]));
+    *reinterpret_cast<__half *>(p + P::v_scale(tok, g)) = s;
+    *reinterpret_cast<__half *>(p + P::v_zero(tok, g)) = z;
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<uint32_t *>(p + P::k_word(tok, 4 * g + x)) =
+          four(c[8 * x], c[8 * x + 2], c[8 * x + 4], c[8 * x + 6]) +
+          (four(c[8 * x + 1], c[8 * x + 3], c[8 * x + 5], c[8 * x + 7]) << 16);
+    *reinterpret_cast<__half *>(p + P::k_scale(tok, g)) = s;
+    *reinterpret_cast<__half *>(p + P::k_zero(tok, g)) = z;
   }
 }
 
+// Two codes (bits 0-3 of the halves of w) as a pair of T: code * s + z.
+template <typename T>
+__device__ __forceinline__ uint32_t values(uint32_t w, uint64_t s2, uint64_t z2) {
+  const uint32_t h = w & 0x000f000fu;
+  // Integers under the exponent of 2^23, less 2^23: no conversion instruction.
+  const float a = __uint_as_float(0x4b000000u | (h & 15u)) - 8388608.f;
+  const float b = __uint_as_float(0x4b000000u | (h >> 16)) - 8388608.f;
+  float x, y;
+  f2_unpack(f2_fma(f2_pack(a, b), s2, z2), x, y);
+  return Pack2<T>::pack(x, y);
+}
+
+// A lane per 8 channels of both rows.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const Args a, uint32_t rows) {
   using P = Piece<D>;
@@ -163,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const Args a, uint
   const int x = threadIdx.x % LANES;
   const int64_t slot = __ldg(a.slots + t);
   if (slot >= a.num_slots) atomicCAS(&g_kv4_status, 0, TLLM_DEV_BAD_INDEX);
-  float kf[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, vf[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  uint4 ko = make_uint4(0u, 0u, 0u, 0u), vo = ko;
   if (slot >= 0 && slot < a.num_slots) {
     const uint8_t *p = piece_of(a, slot, h, P::BYTES);
     const int tok = static_cast<int>(slot & (kPieceTokens - 1));
@@ -171,27 +222,25 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const Args a, uint
     const uint32_t kc = *reinterpret_cast<const uint32_t *>(p + P::k_word(tok, x));
     const uint32_t v0 = *reinterpret_cast<const uint16_t *>(p + P::v_bits(tok, g, n));
     const uint32_t v1 = *reinterpret_cast<const uint16_t *>(p + P::v_bits(tok, g, n + 1));
-    const uint32_t vc = v0 | (v1 << 16);
     const float ks = __half2float(*reinterpret_cast<const __half *>(p + P::k_scale(tok, g)));
     const float kz = __half2float(*reinterpret_cast<const __half *>(p + P::k_zero(tok, g)));
     const float vs = __half2float(*reinterpret_cast<const __half *>(p + P::v_scale(tok, g)));
     const float vz = __half2float(*reinterpret_cast<const __half *>(p + P::v_zero(tok, g)));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      kf[j] = fmaf(static_cast<float>((kc >> (4 * (j >> 1) + 16 * (j & 1))) & 15u), ks, kz);
-      vf[j] = fmaf(static_cast<float>((vc >> (4 * j)) & 15u), vs, vz);
-    }
+    const uint64_t ks2 = f2_pack(ks, ks), kz2 = f2_pack(kz, kz), vs2 = f2_pack(vs, vs), vz2 = f2_pack(vz, vz);
+    ko = make_uint4(values<T>(kc, ks2, kz2), values<T>(kc >> 4, ks2, kz2), values<T>(kc >> 8, ks2, kz2),
+                    values<T>(kc >> 12, ks2, kz2));
+    vo = make_uint4(values<T>(v0 | (v0 << 12), vs2, vz2), values<T>((v0 >> 8) | (v0 << 4), vs2, vz2),
+                    values<T>(v1 | (v1 << 12), vs2, vz2), values<T>((v1 >> 8) | (v1 << 4), vs2, vz2));
   }
-  T *ko = static_cast<T *>(const_cast<void *>(a.k)) + static_cast<int64_t>(t) * a.skt + h * a.skh + 8 * x;
-  T *vo = static_cast<T *>(const_cast<void *>(a.v)) + static_cast<int64_t>(t) * a.svt + h * a.svh + 8 * x;
-  st_stream(ko, pack8<T>(kf));
-  st_stream(vo, pack8<T>(vf));
+  st_stream(static_cast<T *>(const_cast<void *>(a.k)) + static_cast<int64_t>(t) * a.skt + h * a.skh + 8 * x, ko);
+  st_stream(static_cast<T *>(const_cast<void *>(a.v)) + static_cast<int64_t>(t) * a.svt + h * a.svh + 8 * x, vo);
 }
 
 template <typename T, int D>
 int launch(const Args &a, bool append, cudaStream_t st) {
   const int64_t rows = a.T * a.H;
-  const unsigned grid = static_cast<unsigned>((rows * (D / 8) + kThreads - 1) / kThreads);
+  const int lanes = append ? 2 * Piece<D>::W : D / 8;
+  const unsigned grid = static_cast<unsigned>((rows * lanes + kThreads - 1) / kThreads);
   if (append) kv4_append_kernel<T, D><<<grid, kThreads, 0, st>>>(a, static_cast<uint32_t>(rows));
   else kv4_gather_kernel<T, D><<<grid, kThreads, 0, st>>>(a, static_cast<uint32_t>(rows));
   return cuda_status(cudaGetLastError(), append ? "paged kv4 append launch" : "paged kv4 gather launch");
