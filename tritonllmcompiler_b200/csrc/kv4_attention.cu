@@ -36,6 +36,9 @@ constexpr int kTile = 32;   // tokens a warp takes at a time: two pieces
 constexpr int kStages = 2;  // tiles of a warp in shared memory
 constexpr int kMergeLoads = 8;  // parts a merging warp reads at a time
 constexpr int kMinTiles = 2;  // a warp's least run of tiles
+// Places of the line that a segment's queries, results and start take (64 and 300 requests of 512 .. 8192 keys, four
+// of 100,000: none 109, 386 and 192 us, 3 103, 370 and 187, 4 103, 364 and 187, 6 103, 368 and 185).
+constexpr int kExtra = 4;
 constexpr int kSplitRows = 32;  // query rows per sequence and KV head up to which kv4_split_kernel runs
 
 // CTAs of the split kernel per SM: what its registers allow without spilling much (two row tiles of 8 in
@@ -129,14 +132,14 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
     fence_mbar_init();
   }
   int64_t per, total;
-  scan_line<ROWS, kTile>(a, s_line, kMinTiles, per, total, &g_kv4a_status);
+  scan_line<ROWS, kTile, kExtra>(a, s_line, kMinTiles, per, total, &g_kv4a_status);
   clear_rows<T, D>(a);
   const int worker = blockIdx.x * kWarps + warp;
   if (lane == 0) a.ws_open[worker].workers = 0;
   int64_t pos = worker * per;
   const int64_t end = min(pos + per, total);
   Segment sg;
-  if (pos >= end || !first_segment<ROWS, kTile>(a, s_line.seq[warp], s_line.off[warp], end - pos, sg)) return;
+  if (pos >= end || !first_segment<ROWS, kTile, kExtra>(a, s_line.seq[warp], s_line.rt[warp], s_line.off[warp], end - pos, sg)) return;
   const Place &pl = sg.pl;
   bool at_start = true;  // the worker's first segment
 
@@ -488,13 +491,13 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
   // ---- this segment's results; the next one's copies go out first ----
   const Segment done = sg;
   const int64_t done_pos = pos;
-  pos += sg.count;
-  const bool more = next_segment<ROWS, kTile>(a, end - pos, sg);
+  pos += sg.rest;
+  const bool more = next_segment<ROWS, kTile, kExtra>(a, end - pos, sg);
   if (more) prime();
   const bool whole = done.count == done.nt;
   const int64_t slot = 2 * static_cast<int64_t>(worker) + (at_start ? 0 : 1);
   if (!whole && done.first == 0 && lane == 0)
-    a.ws_open[worker] = Open{static_cast<int>((done_pos + done.nt - 1) / per) - worker + 1, static_cast<int>(slot),
+    a.ws_open[worker] = Open{static_cast<int>((done_pos + done.rest - 1) / per) - worker + 1, static_cast<int>(slot),
                              done.hk, done.pl.row0, done.pl.r0, done.pl.nr, 0, 0};
   const float f1 = pow2(24), f2 = pow2(20);  // the units of the two kinds of rows
 #pragma unroll

@@ -77,40 +77,53 @@ __device__ __forceinline__ int key_tiles(const Place &p) {
 }
 
 // All key tiles of all row tiles form one line: sequences, in them row tiles of ROWS rows, in them KV
-// heads, in them tiles of TILE keys. Each worker takes an equal run of it (within a tile), whatever
-// the lengths are; a run's parts of one row tile are its segments.
+// heads, in them EXTRA places for what a row tile costs besides its keys (queries, results, the way
+// there) and then tiles of TILE keys. Each worker takes an equal run of it (within a place), whatever the
+// lengths are; a run's parts of one row tile are its segments.
 struct Segment {
   Place pl;
   int hk, nt;        // KV head; key tiles of the row tile
   int first, count;  // the segment's key tiles
+  int rest;          // places from the segment's start to the end of the row tile
 };
 
 template <int THREADS, int WPC>
 struct LineScan {
   int64_t warp[THREADS / 32];
-  int64_t off[WPC];  // tiles before the run's start in its sequence
-  int seq[WPC];
+  int64_t off[WPC];  // places before the run's start in its row tile (of all KV heads)
+  int seq[WPC], rt[WPC];
 };
 
-template <int ROWS, int TILE>
-__device__ __forceinline__ int64_t tiles_of_sequence(const Args &a, int b, int *status) {
-  int64_t t = 0;
-  Place p;
-  for (int rt = 0; rt < a.n_rt && locate<ROWS>(a, b, rt, p); ++rt) t += key_tiles<TILE>(p);
-  if (p.n_q > a.max_new) atomicCAS(status, 0, TLLM_DEV_BAD_INDEX);
-  return t * a.Hkv;
-}
-
-// Finds the runs of the CTA's WPC workers: a scan over the sequences, done by every CTA, so that it
-// needs no launch of its own. All threads; leaves with the CTA synchronised.
-template <int ROWS, int TILE, int THREADS, int WPC>
+// Finds the runs of the CTA's WPC workers: a scan over all sequences' row tiles, done by every CTA, so that
+// it needs no launch of its own (a thread per row tile: per sequence, 16 row tiles in turn took 4 us). All
+// threads; leaves with the CTA synchronised.
+template <int ROWS, int TILE, int EXTRA, int THREADS, int WPC>
 __device__ __forceinline__ void scan_line(const Args &a, LineScan<THREADS, WPC> &s, int min_tiles, int64_t &per,
                                           int64_t &total, int *status) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int share = (a.B + THREADS - 1) / THREADS;
-  const int b0 = min(tid * share, a.B), b1 = min(b0 + share, a.B);
+  const int64_t n = static_cast<int64_t>(a.B) * a.n_rt, share = (n + THREADS - 1) / THREADS;
+  const int64_t i0 = min(tid * share, n);
+  const int count = static_cast<int>(min(share, n - i0)), first_b = static_cast<int>(i0 / a.n_rt);
+  const int first_rt = static_cast<int>(i0 - static_cast<int64_t>(first_b) * a.n_rt);
+  // Calls visit(b, rt, places) for this thread's row tiles until it returns false.
+  auto each = [&](auto visit) {
+    int b = first_b, rt = first_rt;
+    for (int i = 0; i < count; ++i) {
+      Place p;
+      const int64_t places = locate<ROWS>(a, b, rt, p) ? static_cast<int64_t>(key_tiles<TILE>(p) + EXTRA) * a.Hkv : 0;
+      if (rt == 0 && p.n_q > a.max_new) atomicCAS(status, 0, TLLM_DEV_BAD_INDEX);
+      if (!visit(b, rt, places)) return;
+      if (++rt == a.n_rt) {
+        rt = 0;
+        ++b;
+      }
+    }
+  };
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of_sequence<ROWS, TILE>(a, b, status);
+  each([&](int, int, int64_t places) {
+    mine += places;
+    return true;
+  });
   int64_t upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -129,44 +142,39 @@ __device__ __forceinline__ void scan_line(const Args &a, LineScan<THREADS, WPC> 
   for (int w = 0; w < WPC; ++w) {
     int64_t off = (static_cast<int64_t>(blockIdx.x) * WPC + w) * per - (upto - mine);
     if (off < 0 || off >= mine) continue;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t t = tiles_of_sequence<ROWS, TILE>(a, b, status);
-      if (off < t) {
+    each([&](int b, int rt, int64_t places) {
+      if (off < places) {
         s.seq[w] = b;
+        s.rt[w] = rt;
         s.off[w] = off;
-        break;
+        return false;
       }
-      off -= t;
-    }
+      off -= places;
+      return true;
+    });
   }
   __syncthreads();
 }
 
-// The segment that starts `off` tiles into sequence b; false past the last sequence, which cannot
-// be while lengths stay as they were scanned.
-template <int ROWS, int TILE>
-__device__ __forceinline__ bool first_segment(const Args &a, int b, int64_t off, int64_t left, Segment &g) {
-  for (int rt = 0; b < a.B;) {
-    if (locate<ROWS>(a, b, rt, g.pl)) {
-      g.nt = key_tiles<TILE>(g.pl);
-      if (off < static_cast<int64_t>(g.nt) * a.Hkv) {
-        g.hk = static_cast<int>(off / g.nt);
-        g.first = static_cast<int>(off % g.nt);
-        g.count = static_cast<int>(min(static_cast<int64_t>(g.nt - g.first), left));
-        return true;
-      }
-      off -= static_cast<int64_t>(g.nt) * a.Hkv;
-    }
-    if (++rt == a.n_rt) {
-      rt = 0;
-      ++b;
-    }
-  }
-  return false;
+// The segment that starts `off` places into row tile rt of sequence b; false if the run ends before its keys
+// (the next worker has them all), or if there is none (not while lengths stay as they were scanned).
+template <int ROWS, int TILE, int EXTRA>
+__device__ __forceinline__ bool first_segment(const Args &a, int b, int rt, int64_t off, int64_t left, Segment &g) {
+  if (!locate<ROWS>(a, b, rt, g.pl)) return false;
+  g.nt = key_tiles<TILE>(g.pl);
+  const int places = g.nt + EXTRA;
+  g.hk = static_cast<int>(off / places);
+  if (g.hk >= a.Hkv) return false;
+  const int at = static_cast<int>(off % places);
+  g.first = max(at - EXTRA, 0);
+  g.rest = places - at;
+  g.count = static_cast<int>(min(static_cast<int64_t>(g.nt - g.first), left - max(EXTRA - at, 0)));
+  return g.count > 0;
 }
 
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, int EXTRA>
 __device__ __forceinline__ bool next_segment(const Args &a, int64_t left, Segment &g) {
+  left -= EXTRA;
   if (left <= 0) return false;
   g.first = 0;
   if (++g.hk == a.Hkv) {
@@ -181,6 +189,7 @@ __device__ __forceinline__ bool next_segment(const Args &a, int64_t left, Segmen
     } while (!locate<ROWS>(a, b, rt, g.pl));
     g.nt = key_tiles<TILE>(g.pl);
   }
+  g.rest = g.nt + EXTRA;
   g.count = static_cast<int>(min(static_cast<int64_t>(g.nt), left));
   return true;
 }
