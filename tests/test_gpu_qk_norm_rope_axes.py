@@ -152,3 +152,14 @@ def test_refused_arguments(cuda_device):
     for sections, mix in (((16, 17), False), ((8,) * 5, False), ((33, -1), True)):
         with pytest.raises(AssertionError):
             qk_norm_rope(q, k, wq, wk, cos, sin, pos.expand(len(sections), -1), sections=sections, interleaved=mix)
+
+
+# Enough rows that a lane group takes 8, 4 and 2 heads (the last group of a block is not full in one).
+@pytest.mark.parametrize("T,hq,hkv,D,sections,mix,dtype", [
+    (1901, 32, 8, 128, (16, 24, 24), False, torch.bfloat16),
+    (2503, 12, 4, 128, (64,), False, torch.float16),
+    (5003, 6, 2, 64, (12, 10, 10), True, torch.bfloat16),
+])
+def test_many_rows(cuda_device, T, hq, hkv, D, sections, mix, dtype):
+    test_forward(cuda_device, T, hq, hkv, D, sections, mix, dtype)
+    test_backward(cuda_device, T, hq, hkv, D, sections, mix, dtype)

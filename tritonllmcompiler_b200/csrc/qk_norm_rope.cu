@@ -284,11 +284,13 @@ int heads_per_group(const Args &a, int64_t D, int most, int64_t full) {
 
 template <typename T, int D>
 int forward_d(const Args &a, cudaStream_t st) {
-  const int R = heads_per_group(a, D, 4, 512);
+  // (16,384 tokens of 40 heads of 128: four heads a lane group 78 us, eight 71.)
+  const int R = heads_per_group(a, D, 8, 512);
   const int64_t groups = a.T * ((a.part[0].H + a.part[1].H) / R);
   const unsigned grid = static_cast<unsigned>((groups * (D / 16) + kThreads - 1) / kThreads);
   const uint32_t g = static_cast<uint32_t>(groups);
-  if (R == 4) qk_norm_rope_kernel<T, D, 4><<<grid, kThreads, 0, st>>>(a, g);
+  if (R == 8) qk_norm_rope_kernel<T, D, 8><<<grid, kThreads, 0, st>>>(a, g);
+  else if (R == 4) qk_norm_rope_kernel<T, D, 4><<<grid, kThreads, 0, st>>>(a, g);
   else if (R == 2) qk_norm_rope_kernel<T, D, 2><<<grid, kThreads, 0, st>>>(a, g);
   else qk_norm_rope_kernel<T, D, 1><<<grid, kThreads, 0, st>>>(a, g);
   return cuda_status(cudaGetLastError(), "qk_norm_rope launch");
