@@ -39,7 +39,10 @@ constexpr int kMinTiles = 2;  // a warp's least run of tiles
 // Places of the line that a segment's queries, results and start take (64 and 300 requests of 512 .. 8192 keys, four
 // of 100,000: none 109, 386 and 192 us, 3 103, 370 and 187, 4 103, 364 and 187, 6 103, 368 and 185).
 constexpr int kExtra = 4;
-constexpr int kSplitRows = 32;  // query rows per sequence and KV head up to which kv4_split_kernel runs
+// Query rows per sequence and KV head up to which kv4_split_kernel runs. 64 requests of 512 .. 8192 keys, split
+// and prefill kernel: 16 rows 159 and 259 us, 32 rows 294 and 261, 48 rows 421 and 263; four of 100,000 keys,
+// 32 rows: 271 and 290.
+constexpr int kSplitRows = 32;
 
 // CTAs of the split kernel per SM: what its registers allow without spilling much (two row tiles of 8 in
 // 168 registers, three CTAs, took 175 us where 157 do; one in 128, four CTAs, 135 where 123 did).
@@ -111,6 +114,10 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 // range whatever the size of V (from the largest scale met), and m follows the maximum only
 // when it grows by more than 2^3 (weights and products stay under 2^15).
 // An S^T result becomes a P^T operand by transposing 8 x 8 blocks in registers (movmatrix).
+//
+// Bound: HBM by bytes (1.25 D per token and head), but what holds it now is turning codes into operands:
+// 64 decode steps of U[512, 8192] keys, 32 heads over 8 of 128, fp16: 99 us, 3.9 TB/s; four requests of
+// 65,536 .. 131,072 keys with up to 32 rows: 182 us, half of the issue slots and 39 % of the tensor pipe.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const Args a) {
   using P = Piece<D>;
