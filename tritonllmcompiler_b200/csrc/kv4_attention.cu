@@ -116,8 +116,8 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 // An S^T result becomes a P^T operand by transposing 8 x 8 blocks in registers (movmatrix).
 //
 // Bound: HBM by bytes (1.25 D per token and head), but what holds it now is turning codes into operands:
-// 64 decode steps of U[512, 8192] keys, 32 heads over 8 of 128, fp16: 99 us, 3.9 TB/s; four requests of
-// 65,536 .. 131,072 keys with up to 32 rows: 182 us, half of the issue slots and 39 % of the tensor pipe.
+// 64 decode steps of U[512, 8192] keys, 32 heads over 8 of 128, fp16: 101 us, 3.9 TB/s; four requests of
+// 65,536 .. 131,072 keys with up to 32 rows: 180 us, half of the issue slots and 39 % of the tensor pipe.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const Args a) {
   using P = Piece<D>;

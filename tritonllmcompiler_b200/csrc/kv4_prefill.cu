@@ -18,7 +18,7 @@
 //
 // Bound: tensor products, 4 Hq D flops per visible pair, if K and V were 16-bit. They are 4-bit, so each tile
 // of 128 keys is unpacked for every 128 rows: 8 requests of up to 512 new tokens in up to 4096, 32 heads over
-// 8 of 128, bf16: 184 us, 454 TFLOP/s. A tile takes 3200 cycles, 2800 of them each for its softmax and,
+// 8 of 128, bf16: 183 us, 458 TFLOP/s. A tile takes 3200 cycles, 2800 of them each for its softmax and,
 // beside it, its unpacking; half of the issue slots, 42 % of the integer pipe and a quarter of the tensor
 // pipe are busy, so latency between few warps holds it. What was slower on the same requests: part of the powers
 // of two by a polynomial (+9 to 15 %), twice the unpacking warps (+15 %), a row's 64 scores in registers at
