@@ -205,6 +205,16 @@ def test_attention(cuda_device, lens, new, hkv, G, D, bs, dtype):
     _check(case, lens, new, bs, dtype)
 
 
+# Many short requests: runs of the line start and end everywhere in their row tiles, before the first key too.
+@pytest.mark.parametrize("B,longest,most,hkv,G,D,dtype", [
+    (250, 200, 1, 4, 4, 64, F), (300, 400, 4, 2, 4, 128, BF), (100, 500, 40, 2, 4, 128, BF), (61, 150, 150, 3, 2, 64, F)])
+def test_many_requests(cuda_device, B, longest, most, hkv, G, D, dtype):
+    rng = np.random.default_rng(B)
+    new = [int(n) for n in rng.integers(0, most + 1, B)]
+    lens = [int(rng.integers(n, longest + 1)) for n in new]
+    _check(_case(B, lens, new, hkv, G, D, 16, dtype), lens, new, 16, dtype)
+
+
 @pytest.mark.parametrize("lens,new,G,D", [([50, 130, 5], [3, 20, 5], 4, 128), ([300, 40], [150, 2], 2, 64)])
 def test_attention_not_causal(cuda_device, lens, new, G, D):
     _check(_case(5, lens, new, 2, G, D, 16, F), lens, new, 16, F, causal=False)
