@@ -93,6 +93,9 @@ def quantise(x):
     with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
         s = ((hi - lo) * np.float32(1 / 15)).astype(np.float16)
         z = lo.astype(np.float16)
+        # a rounded-up scale must not put the largest code past fp16's range
+        past = (hi < 65520) & (15 * np.float32(s) + np.float32(z) >= 65520)
+        s = np.where(past, np.nextafter(s, np.float16(0)), s)
         sf, zf = np.float32(s), np.float32(z)
         inv = np.where(sf > 0, np.float32(1) / sf, np.float32(0))
         codes = np.clip(np.rint((g - zf) * inv), 0, 15)

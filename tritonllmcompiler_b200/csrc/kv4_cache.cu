@@ -3,7 +3,9 @@
 //
 // A group of 32 channels x of one token and head becomes
 //   s = fp16((max - min) * (1 / 15)), z = fp16(min), code = clamp(rint((x - z) * (s > 0 ? 1 / s : 0)), 0, 15),
-// each step one IEEE fp32 operation (no contraction), so the codes do not depend on the compiler.
+// each step one IEEE fp32 operation (no contraction), so the codes do not depend on the compiler. Where
+// all of the group is within fp16's range but 15 s + z rounds past its end (a scale that was rounded up), s is
+// one fp16 step less, so that every code stands for a number of that range.
 // s and z are fp16: 11 bits put the reconstruction within 1 / 2048 of the group's range of where
 // exact ones would, a fraction of the half step of 1 / 30, for 4 bytes per 16 bytes of codes. A
 // group with a NaN or an infinity, or beyond fp16's range, reads back as NaN or infinities.
@@ -87,6 +89,8 @@ constexpr float kRound = 12582912.f;  // 1.5 * 2^23: y + kRound has y, rounded t
 constexpr uint32_t kRoundBits = 0x4b400000u;
 constexpr uint32_t kRoundFour = kRoundBits * 0x1111u;
 
+constexpr float kPastHalf = 65520.f;  // rounds to infinity in fp16
+
 // A group's 32 channels, two a word: its scale and zero, and sums[i] = kRoundBits + code i.
 template <typename T>
 __device__ __forceinline__ void quantise(const uint32_t (&w)[16], __half &s, __half &z, uint32_t (&sums)[32]) {
@@ -105,7 +109,9 @@ __device__ __forceinline__ void quantise(const uint32_t (&w)[16], __half &s, __h
   const float hi = h.x >= h.y ? h.x : (h.y > h.x ? h.y : __fadd_rn(h.x, h.y));
   s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   z = __float2half_rn(lo);
-  const float sf = __half2float(s), zf = __half2float(z);
+  const float zf = __half2float(z);
+  if (hi < kPastHalf && __fmaf_rn(15.f, __half2float(s), zf) >= kPastHalf) s = __ushort_as_half(__half_as_ushort(s) - 1);
+  const float sf = __half2float(s);
   const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
   // All steps are monotonic: if the ends stay inside, so does everything between.
   const bool inside = __fmul_rn(__fsub_rn(lo, zf), inv) >= -0.5f && __fmul_rn(__fsub_rn(hi, zf), inv) < 15.5f;

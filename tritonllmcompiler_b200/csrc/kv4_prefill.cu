@@ -13,8 +13,9 @@
 //                 two that keeps them in its range), softmax with a lazy rescale of O (2^8), results
 // V's columns are stored in the order 0 4 1 5 2 6 3 7 of every eight channels (the order in which one
 // mask yields pairs) and put right where O is read. The V rows of a last tile past the context are
-// zeros. A V group whose scale or zero is no number is stored as zeros too and noted in a mask per token,
-// and the rows that see the token get NaN in its channels: a product would spread it to rows that do not.
+// zeros. A V group whose scale, zero or largest value (15 s + z) is no fp16 number is stored as zeros too and
+// noted in a mask per token, and the rows that see the token get NaN in its channels: a product would spread it to
+// rows that do not.
 //
 // Bound: tensor products, 4 Hq D flops per visible pair, if K and V were 16-bit. They are 4-bit, so each tile
 // of 128 keys is unpacked for every 128 rows: 8 requests of up to 512 new tokens in up to 4096, 32 heads over
@@ -138,6 +139,12 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t s, uint32_t z, 
   for (int i = 0; i < 4; ++i) x[i] = fma_half2(x[i], s, z);
 }
 
+constexpr uint32_t kFifteen = 0x4b804b80u;  // the largest code, in fp16
+// Pieces in which a V scale or zero has at least this size (2184) have their groups looked at one by one: below
+// it, 15 s + z is less than 16 * 2184 and a number. (Each lane over all its groups in registers, eight times
+// the code: 199 us where a lane per group, through shared memory, takes 184 on the requests above.)
+constexpr uint32_t kLook = 0x6844u;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) {
   using P = Piece<D>;
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         const uint32_t st = it & 1, empty = ((it >> 1) & 1) ^ 1, rst = it % kRawStages;
         // Tokens of this warp's piece that are keys (the others were not loaded, or hold anything).
         const int valid = min(max(sg.pl.seen - (sg.first + j) * BN - piece * kPieceTokens, 0), kPieceTokens);
-        const uint8_t *raw = smem + G::RAW_OFF + rst * G::RAW_BYTES + piece * P::BYTES;
+        uint8_t *raw = smem + G::RAW_OFF + rst * G::RAW_BYTES + piece * P::BYTES;
         ok = __all_sync(0xffffffffu, wait(&raw_full[rst], (it / kRawStages) & 1, SITE_RAWFULL) && wait(&k_empty[st], empty, SITE_KEMPTY));
         if (!ok) break;
         if (valid > 0) {
@@ -277,22 +284,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
           }
           // Tokens past the last key, or some value that is no number: zeros, and a note of the latter.
           uint32_t bad = 0;  // bits g: token 2 pr, bits 8 + g: the next one
-          const bool odd = valid < kPieceTokens || max(big & 0xffffu, big >> 16) >= 0x7c00u;
+          const bool odd = valid < kPieceTokens || max(big & 0xffffu, big >> 16) >= kLook;
           const bool any_odd = __any_sync(0xffffffffu, odd);
           if (any_odd) {
-#pragma unroll
-            for (int g = 0; g < W; ++g)
-#pragma unroll
+            __syncwarp();
+            if (m < W) {  // of the lanes that share two tokens, each looks at a group
+#pragma unroll 1
               for (int e = 0; e < 2; ++e) {
-                const int sh_s = 16 * (g & 1), sh_z = 16 * e;
-                const uint32_t s1 = (sc[e * (W / 2) + g / 2] >> sh_s) & 0x7fffu, z1 = (ze[g] >> sh_z) & 0x7fffu;
-                const bool past = 2 * pr + e >= valid, none = s1 >= 0x7c00u || z1 >= 0x7c00u;
-                if (!past && none) bad |= 1u << (8 * e + g);
-                if (past || none) {
-                  sc[e * (W / 2) + g / 2] &= ~(0xffffu << sh_s);
-                  ze[g] &= ~(0xffffu << sh_z);
-                }
+                uint16_t *sp = reinterpret_cast<uint16_t *>(raw + P::v_scale(2 * pr + e, m));
+                uint16_t *zp = reinterpret_cast<uint16_t *>(raw + P::v_zero(2 * pr + e, m));
+                const uint32_t top = fma_half2(*sp, kFifteen, *zp);
+                const bool past = 2 * pr + e >= valid;
+                const bool none = (*zp & 0x7fffu) >= 0x7c00u || (top & 0x7fffu) >= 0x7c00u;
+                if (!past && none) bad |= 1u << (8 * e + m);
+                if (past || none) *sp = *zp = 0;
               }
+            }
+            bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+            bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+            __syncwarp();
+            load_words<W>(raw + P::v_scale(2 * pr, 0), sc);
+#pragma unroll
+            for (int g = 0; g < W; ++g) ze[g] = *reinterpret_cast<const uint32_t *>(raw + P::v_zero(2 * pr, g));
           }
 #pragma unroll
           for (int g = 0; g < W; ++g) {
