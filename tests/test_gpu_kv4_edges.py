@@ -88,3 +88,40 @@ def test_fp16_groups_stay_in_fp16(cuda_device):
         # half a step, 15 steps of the scale's rounding (2^-10 at most), and fp16's
         err = (got.cpu().double() - want.double()).abs()
         assert (err <= step * (0.5 + 15 * 2.0 ** -10) + 2.0 ** -11 * want.double().abs()).all()
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("length", [64, 65, 96, 128, 129])
+@pytest.mark.parametrize("lo,hi", [(-70000, -70000), (-70000, 0), (70000, 70000)])
+def test_zeros_beyond_fp16(cuda_device, lo, hi, length, new):
+    """A V group with finite scale whose zero is no fp16 number gives no numbers to the rows that see its
+    token, wherever in a tile the context ends, and nothing to the others."""
+    case = _case(21, [length], [new], 1, 4, 128, 16, BF)
+    before = _attend(case, [new], 16)
+    v = torch.randn(1, 128, generator=torch.Generator().manual_seed(2))
+    v[0, 32:64] = torch.linspace(lo, hi, 32)
+    _newest(case, 16, v=v.to(BF))
+    got = _attend(case, [new], 16)
+    assert torch.equal(got[:-1], before[:-1])
+    assert not got[-1, :, 32:64].isfinite().any()
+    assert got[-1, :, :32].isfinite().all() and got[-1, :, 64:].isfinite().all()
+
+
+@pytest.mark.parametrize("scale,zero", [(float("inf"), 1.0), (float("nan"), 1.0), (1.0, float("nan")), (8000.0, 60000.0)])
+@pytest.mark.parametrize("D,new", [(64, [1, 3]), (128, [6, 3]), (128, [2, 1])])
+def test_any_group_without_numbers_is_hidden(cuda_device, D, new, scale, zero):
+    """Scales and zeros of any kind in the newest token and in the next slot, which is no key: the
+    first reach the row that sees them, the others no row, whatever the weights are."""
+    lens, G, W = [90, 33], 4, D // 32
+    case = _case(27, lens, new, 1, G, D, 16, F)
+    before = _attend(case, new, 16)
+    for b in (0, 1):
+        page = int(case[2][b, lens[b] // 16])
+        t = lens[b] % 16
+        for token in ((t - 1, t) if b == 0 else (t,)):
+            for value, at in ((scale, 18 * D + 2 * (token * W)), (zero, 19 * D + 2 * token)):
+                case[1][page, 0, 0, at:at + 2] = torch.tensor([value], dtype=F).view(torch.uint8).cuda()
+    got = _attend(case, new, 16)
+    last = new[0] - 1
+    assert torch.equal(got[:last], before[:last]) and torch.equal(got[new[0]:], before[new[0]:])
+    assert not got[last, :, :32].isfinite().any() and got[last, :, 32:].isfinite().all()

@@ -65,9 +65,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// All ones in the halves of v that are +0 (as the weights of hidden tokens are).
-__device__ __forceinline__ uint32_t zero_halves(uint32_t v) { return __vcmpeq2(v, 0u); }
-
 // v[r % W] without an indexed register.
 template <int W>
 __device__ __forceinline__ uint32_t pick(const uint32_t (&v)[W], int r) {
@@ -279,13 +276,28 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
   auto tile = [&](uint8_t *base, int at, auto mask_tag) {
     constexpr bool kMask = decltype(mask_tag)::value;
     if constexpr (kMask) {
-      // Slots past the last key may hold anything: their V scales and zeros become 0.
-      if (at + lane >= pl.seen) {
-        uint8_t *pb = base + (lane >> 4) * P::BYTES;
+      // Slots past the last key may hold anything, and a group without numbers must not reach rows that do not
+      // see its token (0 times infinity is no number): their V scales and zeros become 0, and the rows that
+      // see the token get NaN, through the sum that all channels of the group have.
+      const bool past = at + lane >= pl.seen;
+      uint8_t *pb = base + (lane >> 4) * P::BYTES;
+      uint32_t none = 0;
 #pragma unroll
-        for (int g = 0; g < W; ++g) {
-          *reinterpret_cast<uint16_t *>(pb + P::v_scale(lane & 15, g)) = 0;
-          *reinterpret_cast<uint16_t *>(pb + P::v_zero(lane & 15, g)) = 0;
+      for (int g = 0; g < W; ++g) {
+        uint16_t *sp = reinterpret_cast<uint16_t *>(pb + P::v_scale(lane & 15, g));
+        uint16_t *zp = reinterpret_cast<uint16_t *>(pb + P::v_zero(lane & 15, g));
+        const bool number = (fma_half2(*sp, 0x4800u, *zp) & 0x7fffu) < 0x7c00u;  // z + 8 s
+        if (!past && !number) none |= 1u << g;
+        if (past || !number) *sp = *zp = 0;
+      }
+      for (uint32_t left = __ballot_sync(0xffffffffu, none != 0); left != 0; left &= left - 1) {
+        const int t = __ffs(left) - 1;
+        if ((__shfl_sync(0xffffffffu, none, t) >> (r % W)) & 1u) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (at + t < lim[j][c]) accz[j][c] = __int_as_float(0x7fc00000);
         }
       }
       __syncwarp();
@@ -412,10 +424,6 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
       uint32_t z0 = *reinterpret_cast<const uint32_t *>(zp), z1 = *reinterpret_cast<const uint32_t *>(zp + 16);
       z0 = fma_half2(pick<W>(s0, r), 0x48004800u, z0);  // z + 8 s
       z1 = fma_half2(pick<W>(s1, r), 0x48004800u, z1);
-      if constexpr (kMask) {  // no number: left to the rows that see the token (their weights say so)
-        z0 &= ~__vcmpeq2(z0 & 0x7c007c00u, 0x7c007c00u);
-        z1 &= ~__vcmpeq2(z1 & 0x7c007c00u, 0x7c007c00u);
-      }
       const uint8_t *vp = pb + P::V_CODES + cq * D + (r ^ P::swizzle(cq)) * P::CHUNK;
       uint32_t v0[W], v1[W];
       load_words<W>(vp, v0);
@@ -446,20 +454,12 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          uint32_t w0 = mul_half2(b0[j], s0[g]), w1 = mul_half2(b1[j], s1[g]);
-          if constexpr (kMask) {  // a hidden token's scale may be no number
-            w0 &= ~zero_halves(b0[j]);
-            w1 &= ~zero_halves(b1[j]);
-          }
+          const uint32_t w0 = mul_half2(b0[j], s0[g]), w1 = mul_half2(b1[j], s1[g]);
           mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], w0, w1);
           mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], w0, w1);
           if constexpr (kLow) {  // what the products' rounding left out, exactly
-            uint32_t r0 = fma_half2(b0[j], s0[g], w0 ^ 0x80008000u);
-            uint32_t r1 = fma_half2(b1[j], s1[g], w1 ^ 0x80008000u);
-            if constexpr (kMask) {
-              r0 &= ~zero_halves(b0[j]);
-              r1 &= ~zero_halves(b1[j]);
-            }
+            const uint32_t r0 = fma_half2(b0[j], s0[g], w0 ^ 0x80008000u);
+            const uint32_t r1 = fma_half2(b1[j], s1[g], w1 ^ 0x80008000u);
             mma16816(acc[g][0][j], u0[0], u0[1], u1[0], u1[1], r0, r1);
             mma16816(acc[g][1][j], u0[2], u0[3], u1[2], u1[3], r0, r1);
           }
