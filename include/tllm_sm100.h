@@ -491,7 +491,8 @@ TLLM_API int tllm_qk_norm_rope_bwd(const void *dq_out, const void *dk_out, const
  * rows of a block and head contiguous; D 64 or 128, block_size 16, 32 or 64. Each group of 32
  * channels x of a token and head holds scale s = fp16((max - min) / 15) and zero z = fp16(min), and
  * codes c = clamp(rint((x - z) / s), 0, 15), 0 where s is 0; it stands for c * s + z. (s is one fp16 step
- * less where max is below 65520 and 15 s + z is not: every code stands for a number that fp16 has room for.)
+ * less where 15 s + z would round past fp16's largest number, and NaN for a group with a value that fp16 has
+ * no room for, a NaN or an infinity: all of it reads back as NaN, and rows that see it get NaN in its channels.)
  *
  * tllm_paged_kv4_append quantises k and v [T, Hkv, D] (strides sk/sv {token, head}) into slots
  * [T] (block * block_size + offset; negative: skipped; past the pool: skipped and reported through

@@ -96,6 +96,8 @@ def quantise(x):
         # a rounded-up scale must not put the largest code past fp16's range
         past = (hi < 65520) & (15 * np.float32(s) + np.float32(z) >= 65520)
         s = np.where(past, np.nextafter(s, np.float16(0)), s)
+        # nor is a group with a value that fp16 has no room for a group of numbers
+        s = np.where((lo > -65520) & (hi < 65520), s, np.float16(np.nan))
         sf, zf = np.float32(s), np.float32(z)
         inv = np.where(sf > 0, np.float32(1) / sf, np.float32(0))
         codes = np.clip(np.rint((g - zf) * inv), 0, 15)

@@ -125,3 +125,39 @@ def test_any_group_without_numbers_is_hidden(cuda_device, D, new, scale, zero):
     last = new[0] - 1
     assert torch.equal(got[:last], before[:last]) and torch.equal(got[new[0]:], before[new[0]:])
     assert not got[last, :, :32].isfinite().any() and got[last, :, 32:].isfinite().all()
+
+
+def test_groups_beyond_fp16_are_no_numbers(cuda_device):
+    """Groups with a value that fp16 has no room for read back as NaN, whole, also where their scale and zero
+    would be finite; groups that end at its largest bf16 number do not."""
+    x = torch.randn(7, 1, 64, generator=torch.Generator().manual_seed(1))
+    x[0, 0, :32] = torch.linspace(60000, 200000, 32)
+    x[1, 0, :32] = torch.linspace(50000, 100000, 32)
+    x[2, 0, :32] = torch.linspace(-70000, 100, 32)
+    x[3, 0, :32] = -1e5
+    x[4, 0, 5] = float("inf")
+    x[5, 0, 5] = float("nan")
+    x[6, 0, :32] = torch.linspace(-60000, 65280, 32)
+    x = x.to(BF)
+    cache = new_kv4_cache(1, 1, 16, 64)
+    slots = torch.arange(7, dtype=torch.int32).cuda()
+    paged_kv4_append(x.cuda(), -x.cuda(), cache, slots, block_size=16)
+    for got, want in zip(paged_kv4_gather(cache, slots, block_size=16, dtype=BF), (x, -x)):
+        assert got[:6, 0, :32].isnan().all() and got[:6, 0, 32:].isfinite().all() and got[6].isfinite().all()
+        values = torch.from_numpy(O.dequantise(*O.quantise(want.float().numpy()))[0]).to(BF)
+        assert torch.equal(got.cpu().nan_to_num(7.0), values.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("length", [64, 65])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_attention_over_groups_beyond_fp16(cuda_device, which, length, new):
+    """The same NaN from both attention kernels, at any length of the context."""
+    case = _case(28, [length], [new], 1, 4, 64, 16, BF)
+    before = _attend(case, [new], 16)
+    wide = torch.randn(1, 64, generator=torch.Generator().manual_seed(2))
+    wide[0, 32:] = torch.linspace(50000, 100000, 32)
+    _newest(case, 16, **{which: wide.to(BF)})
+    got = _attend(case, [new], 16)
+    assert torch.equal(got[:-1], before[:-1])
+    assert got[-1].isnan().all() if which == "k" else got[-1, :, 32:].isnan().all() and got[-1, :, :32].isfinite().all()

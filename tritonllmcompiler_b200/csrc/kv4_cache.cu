@@ -8,7 +8,9 @@
 // one fp16 step less, so that every code stands for a number of that range.
 // s and z are fp16: 11 bits put the reconstruction within 1 / 2048 of the group's range of where
 // exact ones would, a fraction of the half step of 1 / 30, for 4 bytes per 16 bytes of codes. A
-// group with a NaN or an infinity, or beyond fp16's range, reads back as NaN or infinities.
+// group with a NaN, an infinity or a value that fp16 has no room for gets the scale NaN, so that all of it
+// reads back as NaN, here and in attention: its zero may be finite, and so may both, and then some of what it
+// stands for could be a number in one kernel and none in another.
 //
 // Bound: HBM, 2 bytes in and 0.625 out per element (the other way round when reading back), if the
 // arithmetic stays at a few instructions per element. So a lane that writes holds a whole group of
@@ -110,7 +112,8 @@ __device__ __forceinline__ void quantise(const uint32_t (&w)[16], __half &s, __h
   s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   z = __float2half_rn(lo);
   const float zf = __half2float(z);
-  if (hi < kPastHalf && __fmaf_rn(15.f, __half2float(s), zf) >= kPastHalf) s = __ushort_as_half(__half_as_ushort(s) - 1);
+  if (!(lo > -kPastHalf && hi < kPastHalf)) s = __ushort_as_half(0x7fff);  // NaN
+  else if (__fmaf_rn(15.f, __half2float(s), zf) >= kPastHalf) s = __ushort_as_half(__half_as_ushort(s) - 1);
   const float sf = __half2float(s);
   const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
   // All steps are monotonic: if the ends stay inside, so does everything between.

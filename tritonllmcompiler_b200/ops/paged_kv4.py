@@ -71,8 +71,9 @@ def paged_kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slot
                      *, block_size: int) -> None:
     """Quantises k[t] and v[t] ([T, Hkv, D], fp16 or bf16) into slot slots[t] of the cache, in
     place, for every t with slots[t] >= 0. A slot past the pool is skipped and flagged
-    (``_lib.debug_status()`` returns 0x200). Groups that hold a NaN, an infinity or values beyond
-    fp16's range do not read back as numbers."""
+    (``_lib.debug_status()`` returns 0x200). A group of 32 channels that holds a NaN, an infinity or a
+    value beyond fp16's range reads back as NaN, and so do its channels in the attention of rows that
+    see the token."""
     n, h, d, sc = _check_cache(cache, block_size)
     t = k.shape[0]
     assert k.shape == (t, h, d) and v.shape == k.shape and slots.shape == (t,)
