@@ -57,16 +57,18 @@ class Server:
         self.tables = torch.zeros((requests, max_blocks), dtype=torch.int32, device="cuda")
         self.lens = torch.zeros(requests, dtype=torch.int32, device="cuda")
         self.free = torch.randperm(blocks, device="cuda").int()
-        self.taken = torch.zeros(1, dtype=torch.int64, device="cuda")
+        self.taken = torch.zeros(1, dtype=torch.int32, device="cuda")  # entries of free that are in use
+        # Requests that the pool or their table could not hold at some step: their logits are NaN from there on.
+        self.refused = torch.zeros(requests, dtype=torch.bool, device="cuda")
 
     def step(self, tokens: torch.Tensor, n_new: torch.Tensor, most: int) -> torch.Tensor:
         """Runs the packed new tokens, n_new[b] of request b (at most `most`); returns the logits after
-        each request's last one."""
+        each request's last one, NaN for a request without new tokens or refused."""
         m, bs = self.model, self.block_size
-        # The free list from its first free entry, without learning on the host where that is.
-        index = (self.taken + torch.arange(self.free.shape[0], device="cuda")) % self.free.shape[0]
-        plan = paged_plan(self.tables, self.lens, n_new, self.free[index], block_size=bs, max_tokens=tokens.shape[0])
+        plan = paged_plan(self.tables, self.lens, n_new, self.free, block_size=bs, max_tokens=tokens.shape[0],
+                          free_start=self.taken)
         self.taken += plan.taken
+        self.refused |= plan.new_lens != self.lens + n_new
         self.lens = plan.new_lens.clone()
         x = m.embed[tokens]
         t, hq, hkv = tokens.shape[0], m.heads, m.kv_heads
@@ -79,12 +81,14 @@ class Server:
             x = x + o.view(t, -1) @ layer["out"]
             x = x + swiglu(_norm(x), layer["w1"], layer["w3"]) @ layer["down"]
         last = plan.cu_seqlens[1:].long() - 1
-        return _norm(x[last]).float() @ m.embed.float().T
+        logits = _norm(x[last]).float() @ m.embed.float().T
+        return logits.masked_fill((self.refused | (n_new <= 0))[:, None], float("nan"))
 
 
 def generate(model: Decoder, prompts: list[list[int]], new: int, **how) -> tuple[torch.Tensor, torch.Tensor]:
     """(tokens [requests, new], the logits they were taken from): prompts of any lengths in one step,
-    then a token per request and step."""
+    then a token per request and step. Raises where the pool or a table is too small for that (seen at the
+    end: nothing is read back between the steps)."""
     server = Server(model, len(prompts), **how)
     tokens = torch.tensor([t for p in prompts for t in p], device="cuda")
     n_new = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device="cuda")
@@ -94,6 +98,8 @@ def generate(model: Decoder, prompts: list[list[int]], new: int, **how) -> tuple
         logits.append(server.step(tokens, n_new, most))
         tokens, n_new, most = logits[-1].argmax(-1), one, 1
         out.append(tokens)
+    if server.refused.any():
+        raise RuntimeError(f"the cache cannot hold requests {server.refused.nonzero().flatten().tolist()}")
     return torch.stack(out, 1), torch.stack(logits, 1)
 
 

@@ -448,6 +448,20 @@ TLLM_API int tllm_paged_plan(int32_t *block_tables, const int32_t *seq_lens, con
                              int64_t block_size, const int64_t *sbt, void *stream);
 
 /*
+ * tllm_paged_plan for steps that follow one another: the free list starts after its first
+ * free_start[0] entries (on the device, null: 0), those that earlier steps took. A caller adds
+ * taken[0] to it on the device after each step and reads nothing back; sequences for which the list
+ * has no entries left are refused.
+ */
+TLLM_API int tllm_paged_plan_from(int32_t *block_tables, const int32_t *seq_lens,
+                                  const int32_t *n_new, const int32_t *free_blocks,
+                                  const int32_t *free_start, int32_t *slots, int32_t *positions,
+                                  int32_t *cu_seqlens, int32_t *new_lens, int32_t *taken,
+                                  int64_t B, int64_t max_blocks, int64_t n_free,
+                                  int64_t max_tokens, int64_t block_size, const int64_t *sbt,
+                                  void *stream);
+
+/*
  * RMS norm of every head of q [T, Hq, D] and k [T, Hkv, D] (weights wq, wk [D]) and the rotate-half
  * rotation by positions of 1 to 4 axes, in one pass; a form of rmsnorm_rope
  * (python/triton_llm/ops/rmsnorm_rope.py:51-75) for packed projections, without its rounding of

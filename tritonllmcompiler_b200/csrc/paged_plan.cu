@@ -2,7 +2,8 @@
 //
 // With L_b tokens already in the cache and n_b new ones, sequence b has have_b = ceil(L_b / bs)
 // blocks and takes need_b = ceil((L_b + n_b) / bs) - have_b more from the free list, in order of b:
-// off_b = sum of need over the sequences before it. Packed token i of sequence b is new token
+// off_b = sum of need over the sequences before it (the list starts after the entries that earlier steps
+// took, a count that stays on the GPU too). Packed token i of sequence b is new token
 // t = i - cu[b] at position p = L_b + t, in block j = p / bs: the table's entry where j < have_b,
 // else free[off_b + j - have_b]; its slot is block * bs + p % bs. The thread of a block's first
 // token (p % bs == 0) writes the table entry, so every entry has one writer and no thread reads
@@ -26,6 +27,7 @@ constexpr int64_t kMaxSeqs = 16384;  // the scans of all sequences fit in shared
 struct Args {
   int32_t *block_tables;
   const int32_t *seq_lens, *n_new, *free_blocks;
+  const int32_t *free_start;  // [1]: entries of free_blocks that earlier steps took; null: none
   int32_t *slots, *positions, *cu, *new_lens, *taken;
   int B, n_free, max_tokens, block_size;
   int64_t max_blocks, sbt0, sbt1;
@@ -68,6 +70,9 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Args a) {
   __shared__ int s_taken;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool first = blockIdx.x == 0;  // this CTA also writes the per-sequence results
+  const int start = a.free_start ? min(max(__ldg(a.free_start), 0), a.n_free) : 0;
+  const int32_t *free_blocks = a.free_blocks + start;
+  const int n_free = a.n_free - start;
 
   // Each thread scans a run of consecutive sequences.
   const int per = (a.B + kThreads - 1) / kThreads;
@@ -93,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Args a) {
   int took = 0;
   for (int b = b0; b < b1; ++b) {
     const Seq s = sequence(a, b);
-    const bool ok = s.fits && (s.need == 0 || blk_at + s.need <= a.n_free) &&
+    const bool ok = s.fits && (s.need == 0 || blk_at + s.need <= n_free) &&
                     tok_at + s.n <= a.max_tokens;
     s_cu[b] = sat32(tok_at);
     s_off[b] = ok ? sat32(blk_at) : -1;
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Args a) {
     const int in = static_cast<int>(pos - j * a.block_size);
     const int64_t have = (len + a.block_size - 1) / a.block_size;
     int32_t *entry = a.block_tables + lo * a.sbt0 + j * a.sbt1;
-    const int32_t block = j < have ? *entry : __ldg(a.free_blocks + off + (j - have));
+    const int32_t block = j < have ? *entry : __ldg(free_blocks + off + (j - have));
     if (in == 0) *entry = block;
     a.slots[i] = block < 0 ? -1 : sat32(static_cast<int64_t>(block) * a.block_size + in);
   }
@@ -155,6 +160,18 @@ extern "C" int tllm_paged_plan(int32_t *block_tables, const int32_t *seq_lens,
                                int32_t *taken, int64_t B, int64_t max_blocks, int64_t n_free,
                                int64_t max_tokens, int64_t block_size, const int64_t *sbt,
                                void *stream) {
+  return tllm_paged_plan_from(block_tables, seq_lens, n_new, free_blocks, nullptr, slots, positions,
+                              cu_seqlens, new_lens, taken, B, max_blocks, n_free, max_tokens,
+                              block_size, sbt, stream);
+}
+
+extern "C" int tllm_paged_plan_from(int32_t *block_tables, const int32_t *seq_lens,
+                                    const int32_t *n_new, const int32_t *free_blocks,
+                                    const int32_t *free_start, int32_t *slots, int32_t *positions,
+                                    int32_t *cu_seqlens, int32_t *new_lens, int32_t *taken,
+                                    int64_t B, int64_t max_blocks, int64_t n_free,
+                                    int64_t max_tokens, int64_t block_size, const int64_t *sbt,
+                                    void *stream) {
   using namespace tllm;
   clear_error();
   TLLM_CHECK_ARG(B >= 0 && max_blocks >= 0 && n_free >= 0 && max_tokens >= 0,
@@ -177,6 +194,7 @@ extern "C" int tllm_paged_plan(int32_t *block_tables, const int32_t *seq_lens,
   a.seq_lens = seq_lens;
   a.n_new = n_new;
   a.free_blocks = free_blocks;
+  a.free_start = free_start;
   a.slots = slots;
   a.positions = positions;
   a.cu = cu_seqlens;
