@@ -528,7 +528,8 @@ TLLM_API int tllm_paged_kv4_gather(const void *cache, const int32_t *slots, void
  * h / (Hq / Hkv). Sequence b owns rows cu_seqlens[b] .. cu_seqlens[b + 1] (at most max_new), its
  * newest tokens, already in the cache and counted by context_lens[b]; with causal != 0 a token
  * sees the keys up to its own position, else all of them. Rows that see no key give NaN; rows
- * past cu_seqlens[B] give zeros. Block-table entries outside the pool read block 0 and are
+ * before cu_seqlens[0] or past cu_seqlens[B] give zeros. A sequence with more than max_new tokens is
+ * reported through tllm_debug_status, and its tokens past the first max_new give NaN. Block-table entries outside the pool read block 0 and are
  * reported through tllm_debug_status. workspace: tllm_paged_kv4_attn_workspace_size bytes,
  * 256-byte aligned (0 when no launch splits the keys).
  */

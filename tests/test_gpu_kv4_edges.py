@@ -5,6 +5,7 @@ import torch
 
 from oracle import kv4_oracle as O
 from tests.test_gpu_paged_kv4 import _case, _check
+from tritonllmcompiler_b200 import _lib
 from tritonllmcompiler_b200.ops.paged_kv4 import (new_kv4_cache, paged_attention_kv4,
                                                   paged_kv4_append, paged_kv4_gather)
 
@@ -161,3 +162,37 @@ def test_attention_over_groups_beyond_fp16(cuda_device, which, length, new):
     got = _attend(case, [new], 16)
     assert torch.equal(got[:-1], before[:-1])
     assert got[-1].isnan().all() if which == "k" else got[-1, :, 32:].isnan().all() and got[-1, :, :32].isfinite().all()
+
+
+@pytest.mark.parametrize("new,most", [([5, 1, 9], 4), ([40, 300, 2], 50), ([3, 2, 1], 0), ([1, 70, 1], 1)])
+def test_more_new_tokens_than_promised(cuda_device, new, most):
+    """Flagged; the first max_new tokens of each sequence are what they are, the others NaN (not what the
+    output's memory had), whichever kernel max_new selects."""
+    lens = [60, 400, 33]
+    case = _case(22, lens, new, 2, 4, 64, 16, F)
+    q, cache, table, ctx, cu, _, _ = case
+    whole = _check(case, lens, new, 16, F)
+    torch.full_like(whole, 7.0)  # in the memory that the output gets
+    got = paged_attention_kv4(q.cuda(), cache, table.cuda(), ctx.cuda(), cu.cuda(), most, block_size=16)
+    torch.cuda.synchronize()
+    assert _lib.debug_status() == 0x200
+    for b, n in enumerate(new):
+        r, m = int(cu[b]), min(n, most)
+        # two kernels or two divisions of the keys: each within its bound, some 2^-9 of values of size 4
+        assert ((got[r:r + m].float() - whole[r:r + m].float()).abs() <= 2.0 ** -7).all()
+        assert got[r + m:r + n].isnan().all()
+
+
+@pytest.mark.parametrize("new", [[2, 1], [60, 9]])
+def test_rows_before_the_first_sequence_are_zero(cuda_device, new):
+    """Some sequences of a larger packed batch: the rows of the others are cleared."""
+    lens = [90, 33]
+    q, cache, table, ctx, cu, _, _ = _case(23, lens, new, 1, 4, 128, 16, BF)
+    ref = paged_attention_kv4(q.cuda(), cache, table.cuda(), ctx.cuda(), cu.cuda(), max(new), block_size=16)
+    more = torch.cat([torch.full((21, 4, 128), 3.0, dtype=BF), q, torch.full((5, 4, 128), 3.0, dtype=BF)]).cuda()
+    torch.full_like(more, 7.0)
+    got = paged_attention_kv4(more, cache, table.cuda(), ctx.cuda(), cu.cuda() + 21, max(new), block_size=16)
+    assert (got[:21] == 0).all() and torch.equal(got[21:-5], ref) and (got[-5:] == 0).all()
+    one = paged_attention_kv4(q.cuda(), cache, table.cuda()[1:], ctx.cuda()[1:], cu.cuda()[1:], new[1], block_size=16)
+    assert (one[:new[0]] == 0).all() and ((one[new[0]:].float() - ref[new[0]:].float()).abs() <= 2.0 ** -5).all()
+    assert _lib.debug_status() == 0

@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
     fence_mbar_init();
   }
   int64_t per, total;
-  scan_line<ROWS, kTile, kExtra>(a, s_line, kMinTiles, per, total, &g_kv4a_status);
-  clear_rows<T, D>(a);
+  const bool over = scan_line<ROWS, kTile, kExtra>(a, s_line, kMinTiles, per, total, &g_kv4a_status);
+  other_rows<T, D>(a, over);
   const int worker = blockIdx.x * kWarps + warp;
   if (lane == 0) a.ws_open[worker].workers = 0;
   int64_t pos = worker * per;

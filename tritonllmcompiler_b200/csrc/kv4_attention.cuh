@@ -38,8 +38,8 @@ struct Args {
   float scale_log2;
 };
 
-// A row tile: rows r0 .. r0 + nr of the n_q * G rows of sequence b and a KV head hk, row r being new
-// token r / G of query head hk * G + r % G, and how many keys they see.
+// A row tile: rows r0 .. r0 + nr of the n_q * G rows of sequence b (of those of its first max_new tokens, where it
+// has more) and a KV head hk, row r being new token r / G of query head hk * G + r % G, and how many keys they see.
 struct Place {
   int b, rt, r0, nr, row0, n_q, len, seen;
 };
@@ -56,7 +56,7 @@ __device__ __forceinline__ bool locate(const Args &a, int b, int rt, Place &p) {
   p.row0 = min(max(__ldg(a.cu + b), 0), lim);
   p.n_q = min(max(__ldg(a.cu + b + 1), p.row0), lim) - p.row0;
   p.r0 = rt * ROWS;
-  p.nr = min(ROWS, p.n_q * a.G - p.r0);
+  p.nr = min(ROWS, min(p.n_q, a.max_new) * a.G - p.r0);
   if (p.nr <= 0) return false;
   p.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(a.lens + b), 0)), a.max_blocks << a.log2_bs));
   p.seen = row_keys(a, p, p.r0 + p.nr - 1);
@@ -96,22 +96,26 @@ struct LineScan {
 
 // Finds the runs of the CTA's WPC workers: a scan over all sequences' row tiles, done by every CTA, so that
 // it needs no launch of its own (a thread per row tile: per sequence, 16 row tiles in turn took 4 us). All
-// threads; leaves with the CTA synchronised.
+// threads; leaves with the CTA synchronised. Returns whether some sequence has more than max_new tokens.
 template <int ROWS, int TILE, int EXTRA, int THREADS, int WPC>
-__device__ __forceinline__ void scan_line(const Args &a, LineScan<THREADS, WPC> &s, int min_tiles, int64_t &per,
+__device__ __forceinline__ bool scan_line(const Args &a, LineScan<THREADS, WPC> &s, int min_tiles, int64_t &per,
                                           int64_t &total, int *status) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t n = static_cast<int64_t>(a.B) * a.n_rt, share = (n + THREADS - 1) / THREADS;
   const int64_t i0 = min(tid * share, n);
   const int count = static_cast<int>(min(share, n - i0)), first_b = static_cast<int>(i0 / a.n_rt);
   const int first_rt = static_cast<int>(i0 - static_cast<int64_t>(first_b) * a.n_rt);
+  bool over = false;
   // Calls visit(b, rt, places) for this thread's row tiles until it returns false.
   auto each = [&](auto visit) {
     int b = first_b, rt = first_rt;
     for (int i = 0; i < count; ++i) {
       Place p;
       const int64_t places = locate<ROWS>(a, b, rt, p) ? static_cast<int64_t>(key_tiles<TILE>(p) + EXTRA) * a.Hkv : 0;
-      if (rt == 0 && p.n_q > a.max_new) atomicCAS(status, 0, TLLM_DEV_BAD_INDEX);
+      if (rt == 0 && p.n_q > a.max_new) {
+        atomicCAS(status, 0, TLLM_DEV_BAD_INDEX);
+        over = true;
+      }
       if (!visit(b, rt, places)) return;
       if (++rt == a.n_rt) {
         rt = 0;
@@ -153,7 +157,7 @@ __device__ __forceinline__ void scan_line(const Args &a, LineScan<THREADS, WPC> 
       return true;
     });
   }
-  __syncthreads();
+  return __syncthreads_or(over);
 }
 
 // The segment that starts `off` places into row tile rt of sequence b; false if the run ends before its keys
@@ -194,17 +198,30 @@ __device__ __forceinline__ bool next_segment(const Args &a, int64_t left, Segmen
   return true;
 }
 
-// Rows that belong to no sequence are cleared, by all threads of the grid.
+// Rows from .. to - 1 of the output become `bits`, by threads i0, i0 + step, ...
 template <typename T, int D>
-__device__ __forceinline__ void clear_rows(const Args &a) {
-  const int64_t from = a.B > 0 ? min(max(static_cast<int64_t>(__ldg(a.cu + a.B)), int64_t{0}), a.T) : 0;
+__device__ __forceinline__ void fill_rows(const Args &a, int64_t from, int64_t to, uint32_t bits, int64_t i0, int64_t step) {
   const int hq = a.Hkv * a.G;
-  const int64_t n = (a.T - from) * hq * (D / 8), step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
+  const int64_t n = (to - from) * hq * (D / 8);
+  for (int64_t i = i0; i < n; i += step) {
     const int64_t row = i / (D / 8);
     T *o = static_cast<T *>(a.o) + (from + row / hq) * a.so0 + (row % hq) * a.so1;
-    *reinterpret_cast<uint4 *>(o + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4 *>(o + (i % (D / 8)) * 8) = make_uint4(bits, bits, bits, bits);
   }
+}
+
+// The rows that no row tile has, by all threads of the grid: those before the first sequence and past the last
+// one become zeros, and (over: there are some) those of tokens past a sequence's first max_new NaN.
+template <typename T, int D>
+__device__ __forceinline__ void other_rows(const Args &a, bool over) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  auto row = [&](int b) { return min(max(static_cast<int64_t>(__ldg(a.cu + b)), int64_t{0}), a.T); };
+  fill_rows<T, D>(a, a.B > 0 ? row(a.B) : 0, a.T, 0u, i0, step);
+  if (a.B > 0) fill_rows<T, D>(a, 0, row(0), 0u, i0, step);
+  if (over)
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      fill_rows<T, D>(a, row(b) + a.max_new, row(b + 1), 0x7fff7fffu, threadIdx.x, blockDim.x);
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b) { return Pack2<__half>::pack(a, b); }

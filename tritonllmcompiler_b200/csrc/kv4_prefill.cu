@@ -203,9 +203,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
   }
   tc_fence_before();
   int64_t per, total;
-  scan_line<BM, BN, kExtra>(a, s_line, 1, per, total, &g_kv4p_status);  // (synchronises the CTA)
+  const bool over = scan_line<BM, BN, kExtra>(a, s_line, 1, per, total, &g_kv4p_status);  // (synchronises the CTA)
   tc_fence_after();
-  clear_rows<T, D>(a);
+  other_rows<T, D>(a, over);
   const uint32_t tmem_base = *tmem_holder;
   const uint32_t sQ = smem_u32(smem + G::Q_OFF);
   const uint32_t sK = smem_u32(smem + G::K_OFF);

@@ -120,7 +120,8 @@ def paged_attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_tables: torc
     context_lens[b] - n_b + s; with causal it sees keys up to its own position. Decode is one row
     per sequence; prefill chunks, speculative tokens and idle sequences may be mixed in one call.
     Returns a new [T, Hq, D] tensor: NaN in rows that see no key, as in ``paged_attention``, and
-    zeros in rows past cu_seqlens[B]."""
+    zeros in rows before cu_seqlens[0] or past cu_seqlens[B]. A sequence with more than max_new tokens
+    is flagged (``_lib.debug_status()`` returns 0x200); its tokens past the first max_new give NaN."""
     n, hkv, d, sc = _check_cache(cache, block_size)
     assert q.dim() == 3 and q.shape[2] == d and q.dtype in _lib.DTYPE_CODES
     t, hq, _ = q.shape
