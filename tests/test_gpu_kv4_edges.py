@@ -1,10 +1,13 @@
 """Edges of the serving step over the 4-bit paged cache. Bounds of the attention are those of
 test_gpu_paged_kv4.py unless a test derives its own."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
 from oracle import kv4_oracle as O
-from tests.test_gpu_paged_kv4 import _case, _check
+from tests.test_gpu_paged_kv4 import U, _case, _check, _np
 from tritonllmcompiler_b200 import _lib
 from tritonllmcompiler_b200.ops.paged_kv4 import (new_kv4_cache, paged_attention_kv4,
                                                   paged_kv4_append, paged_kv4_gather)
@@ -196,3 +199,58 @@ def test_rows_before_the_first_sequence_are_zero(cuda_device, new):
     one = paged_attention_kv4(q.cuda(), cache, table.cuda()[1:], ctx.cuda()[1:], cu.cuda()[1:], new[1], block_size=16)
     assert (one[:new[0]] == 0).all() and ((one[new[0]:].float() - ref[new[0]:].float()).abs() <= 2.0 ** -5).all()
     assert _lib.debug_status() == 0
+
+
+def _scores_bounded(q, k, scale, dtype):
+    """Decode over tokens whose K are the rows of k [n, D] (read back from the cache) and V one 1 each,
+    so that the outputs are the weights, against 64 bits.
+
+    Scores may be off by E = 2^-20 of the sizes of their terms, |q| (code s + |z|): the sums of q are held in
+    22 bits, and up to 140 products are added in fp32 or by MMAs that cut off below 2^-23. Each weight changes by
+    a factor within 1 +- 2 E, is rounded to 11 bits, or its product with the scale is (2^-10), and the
+    output once."""
+    n, D = k.shape
+    H = q.shape[0]
+    cache = new_kv4_cache(1, 1, 16, D)
+    v = torch.zeros(n, 1, D, dtype=dtype)
+    for t in range(n):
+        v[t, 0, 32 * (t % (D // 32)):32 * (t % (D // 32)) + 32] = 1  # token t: group t
+    slots = torch.arange(n, dtype=torch.int32).cuda()
+    paged_kv4_append(k[:, None].cuda(), v.cuda(), cache, slots, block_size=16)
+    codes, s, z = O.quantise(k.float().numpy())
+    values, size = O.dequantise(codes, s, z)
+    table, ctx = torch.zeros(1, 1, dtype=torch.int32).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    cu = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    for h in range(0, H, 8):
+        part = q[h:h + 8]
+        got = _np(paged_attention_kv4(part[None].cuda(), cache, table, ctx, cu, 1, block_size=16, sm_scale=scale))[0]
+        x = values @ _np(part).T * scale  # [n, heads]
+        p = np.exp(x - x.max(0))
+        p /= p.sum(0)
+        E = 2.0 ** -20 * scale * (size @ np.abs(_np(part)).T).max(0)
+        for t in range(n):
+            bound = (U[dtype] + 2.0 ** -10 + 2 * E) * p[t] + 2.0 ** -24
+            assert (np.abs(got[:, 32 * t] - p[t]) <= bound).all(), (t, got[:, 32 * t], p[t], bound)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [F, BF])
+def test_scores_of_offset_keys(cuda_device, dtype, D):
+    """Keys far from 0, of opposite sign, under queries whose channels nearly cancel: what is left of a
+    group's sum is a fraction of the unit of the largest element."""
+    rng = np.random.default_rng(3)
+    q = torch.zeros(64, D, dtype=torch.float64)
+    q[:, 2], q[:, 3] = 2.5, -2.5
+    q[:, 4::32] = torch.from_numpy(rng.uniform(0.1, 0.45, (64, 1)) / 2 ** 11)  # (2^12 is 2 to 4 here)
+    k = torch.full((2, D), 500.0)
+    k[1] = -500
+    _scores_bounded(q.to(dtype), k.to(dtype), 1.0, dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [F, BF])
+def test_scores_of_random_keys_with_offsets(cuda_device, dtype, D):
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(64, D, generator=g)
+    k = torch.randn(2, D, generator=g) + 50 * torch.randn(1, D // 32, generator=g).repeat_interleave(32, 1)
+    _scores_bounded(q.to(dtype), k.to(dtype), D ** -0.5, dtype)

@@ -48,6 +48,10 @@ constexpr int kSplitRows = 32;
 // 168 registers, three CTAs, took 175 us where 157 do; one in 128, four CTAs, 135 where 123 did).
 __host__ __device__ constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
 
+// Units of the products with the codes (fp16 subnormals) and with the zeros. The sums of q are split into two fp16
+// parts, 22 bits: in the codes' unit the low part would be a subnormal, and the sum a multiple of half a q unit.
+constexpr float kCodeUnit = 1.f / 16777216.f, kSumUnit = 1.f / 16.f;
+
 enum : int { SITE_TILE = 0x41 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -99,7 +103,8 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 //   q . k = sum_g s_g (sum_{d in g} q_d c_d) + sum_g z_g (sum_{d in g} q_d): one FMA per group and
 //           score on the products' fp32 results; the zeros are one more MMA with the sums of q, held as
 //           high and low fp16 parts. q is brought to [2^12, 2^13) by a power of two per row and is
-//           exact in fp16 from either type, so scores are exact but for fp32 sums.
+//           exact in fp16 from either type (elements 2^-25 of the row's largest or less aside), so scores are
+//           exact but for fp32 sums and the sums' 22 bits: within 2^-20 of the sizes of their terms.
 //   o_d   = sum_t (p_t s_{t,g}) (c_{t,d} - 8) + sum_t p_t (z_{t,g} + 8 s_{t,g}): weights are fp16, and
 //           fp16 again after the scale (packed products on the transposed weights, a third of the
 //           instructions of fp32 ones). The second sum is one more MMA. The 8 centres both sums on
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= pow2(-24);  // the codes' unit; |sum| < 2^-6
+      sum *= kSumUnit;  // |sum| < 2^14
       hi[w] = __half2float(__float2half_rn(sum));
       lo[w] = sum - hi[w];
       // pairs {0,1}, {2,3} 2^-4, {4,5}, {6,7} 2^-4 of channels 32 w + 8 cq
@@ -322,6 +327,8 @@ __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const
       for (int j = 0; j < NT; ++j) {
         x[h][j][0] = x[h][j][1] = x[h][j][2] = x[h][j][3] = 0.f;
         mma16816(x[h][j], z0, z1, 0u, 0u, qs[j], 0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[h][j][i] *= kCodeUnit / kSumUnit;
       }
     }
 #pragma unroll
