@@ -254,3 +254,32 @@ def test_scores_of_random_keys_with_offsets(cuda_device, dtype, D):
     q = torch.randn(64, D, generator=g)
     k = torch.randn(2, D, generator=g) + 50 * torch.randn(1, D // 32, generator=g).repeat_interleave(32, 1)
     _scores_bounded(q.to(dtype), k.to(dtype), D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("log2", [12.0, 16.5, 20.6, -20.6])
+@pytest.mark.parametrize("new", [1, 5, 256])
+def test_many_keys_of_small_weight(cuda_device, new, log2, dtype):
+    """One key of weight 1 and value 0 (first, or with log2 < 0 last of all), thousands of weight 2^-|log2| and
+    value 1: what the rows get is the small weights' sum. Bound as in test_gpu_paged_kv4.py, with the score of
+    the one key, |log2| ln 2, as the size of all terms. A run of a worker holds some 40 tiles here where there
+    are many rows."""
+    n, D, Hkv, G, bs, B = 5000, 64, 8, 4, 64, 2
+    blocks = -(-n // bs)
+    one = 0 if log2 > 0 else n - new
+    k, v = torch.zeros(n, Hkv, D, dtype=dtype), torch.ones(n, Hkv, D, dtype=dtype)
+    k[one], v[one] = 1, 0
+    cache = new_kv4_cache(blocks, Hkv, bs, D)
+    paged_kv4_append(k.cuda(), v.cuda(), cache, torch.arange(n, dtype=torch.int32).cuda(), block_size=bs)
+    table = torch.arange(blocks, dtype=torch.int32).expand(B, -1).cuda()
+    cu = torch.arange(0, B * new + 1, new, dtype=torch.int32).cuda()
+    q = torch.ones(B * new, Hkv * G, D, dtype=dtype, device="cuda")
+    size = abs(log2) * math.log(2)
+    got = _np(paged_attention_kv4(q, cache, table, torch.full((B,), n, dtype=torch.int32).cuda(), cu, new, block_size=bs,
+                                  sm_scale=size / D))
+    small = (n - new + np.arange(new)) * 2.0 ** -abs(log2)  # visible keys but one
+    want = np.tile(small / (1 + small), B)[:, None, None]
+    E = size * (2.0 ** -12 + 2.0 ** -21)
+    assert (np.abs(got - want) <= (U[dtype] + 2.0 ** -10 + 2.0 ** -20 + 2 * E) * want + 2.0 ** -24).all(), \
+        np.abs(got / want - 1).max()
+    assert _lib.debug_status() == 0

@@ -66,6 +66,14 @@ constexpr int TMEM_COLS = 512;
 constexpr int O_COL = 256;  // S buffers at columns [0, 128) and [128, 256)
 constexpr int P_COL = 384;  // P buffers at columns [384, 448) and [448, 512)
 constexpr float kLazyRescaleLog2 = 8.0f;
+// Weights are 2^(x + 7 - m): with the 2^8 that x may grow beyond m they stay within fp16, and those of 2^-21 of the
+// largest keep their 11 bits (without the 2^7, many keys of such weights beside one of weight 1 lost 4 % and more of
+// their sum). Beyond kHuge the 7 would be rounded.
+constexpr float kWeightLog2 = 7.0f;
+constexpr float kHuge = 1048576.f;
+__device__ __forceinline__ float weight_shift(float m) {
+  return m == -INFINITY ? 0.f : (fabsf(m) < kHuge ? kWeightLog2 : 0.f) - m;
+}
 
 enum : int {
   SITE_Q = 0x51,
@@ -525,14 +533,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         if (m_use == -INFINITY) {
           m_use = mx;  // nothing accumulated yet (every earlier P of this row was 0)
         } else if (mx > m_use + kLazyRescaleLog2) {
-          alpha = ex2_approx(m_use - mx);
+          alpha = ex2_approx(weight_shift(mx) - weight_shift(m_use));
           m_use = mx;
           rescale = true;
         }
-        const float neg_m = m_use == -INFINITY ? 0.f : -m_use;
+        const float neg_m = weight_shift(m_use);
         // The exponents below are exact products less the rounded maximum, which is within half an ulp of
-        // its own product; where half an ulp could be many units, round the products first.
-        const bool huge = __any_sync(0xffffffffu, fabsf(m_use) >= 268435456.f && m_use != -INFINITY);
+        // its own product; where that is a good part of a unit and more, round the products first.
+        const bool huge = __any_sync(0xffffffffu, fabsf(m_use) >= kHuge && m_use != -INFINITY);
         const float factor = huge ? 1.f : rs;
         const uint64_t scale2 = f2_pack(factor, factor);
         const uint64_t negm2 = f2_pack(neg_m, neg_m);
@@ -644,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const Args a) 
         mbar_arrive(smem_u32(o_free));
       }
       if (!whole && in && half == 0)
-        a.ws_ml[slot] = make_float2(done_l == 0.f ? -INFINITY : (m_use == -INFINITY ? 0.f : m_use), done_l);
+        a.ws_ml[slot] = make_float2(done_l == 0.f ? -INFINITY : -weight_shift(m_use), done_l);
       if (!whole && done.first == 0 && threadIdx.x == 0)
         a.ws_open[worker] = Open{static_cast<int>((done_pos + done.rest - 1) / per) - worker + 1,
                                  2 * worker + (at_start ? 0 : 1), done.hk, done.pl.row0, done.pl.r0, done.pl.nr, 0, 0};
