@@ -11,6 +11,8 @@ from tests.test_gpu_paged_kv4 import U, _case, _check, _np
 from tritonllmcompiler_b200 import _lib
 from tritonllmcompiler_b200.ops.paged_kv4 import (new_kv4_cache, paged_attention_kv4,
                                                   paged_kv4_append, paged_kv4_gather)
+from tritonllmcompiler_b200.ops.paged_plan import paged_plan
+from tritonllmcompiler_b200.ops.qk_norm_rope import qk_norm_rope
 
 pytestmark = pytest.mark.gpu
 F, BF = torch.float16, torch.bfloat16
@@ -282,4 +284,45 @@ def test_many_keys_of_small_weight(cuda_device, new, log2, dtype):
     E = size * (2.0 ** -12 + 2.0 ** -21)
     assert (np.abs(got - want) <= (U[dtype] + 2.0 ** -10 + 2.0 ** -20 + 2 * E) * want + 2.0 ** -24).all(), \
         np.abs(got / want - 1).max()
+    assert _lib.debug_status() == 0
+
+
+@pytest.mark.parametrize("bad", [torch.float32, torch.float16, torch.float64, torch.bool])
+def test_only_integers_are_indexes(cuda_device, bad):
+    case = _case(24, [20], [2], 1, 2, 64, 16, F)
+    q, cache, table, ctx, cu, k, v = (t.cuda() for t in case)
+    slots = torch.arange(20).cuda()
+    calls = [lambda: paged_kv4_append(k, v, cache, slots.to(bad), block_size=16),
+             lambda: paged_kv4_gather(cache, slots.to(bad), block_size=16)]
+    for i in range(3):
+        a = [table, ctx, cu]
+        a[i] = a[i].to(bad)
+        calls.append(lambda a=a: paged_attention_kv4(q, cache, *a, 2, block_size=16))
+    for i in range(4):
+        a = [ctx, ctx, ctx, ctx]
+        a[i] = a[i].to(bad)
+        calls.append(lambda a=a: paged_plan(table, *a[:3], block_size=16, max_tokens=4, free_start=a[3]))
+    w, cs = torch.ones(64, dtype=F, device="cuda"), torch.ones(32, 32, device="cuda")
+    calls.append(lambda: qk_norm_rope(k, k, w, w, cs, cs, slots.to(bad)))
+    before = cache.clone(), table.clone()
+    for call in calls:
+        with pytest.raises(AssertionError):
+            call()
+    assert torch.equal(cache, before[0]) and torch.equal(table, before[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int16, torch.uint8])
+def test_integers_of_other_sizes(cuda_device, dtype):
+    case = _case(24, [20, 90], [2, 1], 1, 2, 64, 16, F)
+    q, cache, table, ctx, cu, k, v = (t.cuda() for t in case)
+    ref = paged_attention_kv4(q, cache, table, ctx, cu, 2, block_size=16)
+    got = paged_attention_kv4(q, cache, table.to(dtype), ctx.to(dtype), cu.to(dtype), 2, block_size=16)
+    assert torch.equal(got, ref)
+    slots = torch.arange(20, device="cuda")
+    for a, b in zip(paged_kv4_gather(cache, slots.to(dtype), block_size=16), paged_kv4_gather(cache, slots, block_size=16)):
+        assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    w, cs = torch.ones(64, dtype=F, device="cuda"), torch.rand(128, 32, device="cuda")
+    at = torch.arange(110, device="cuda")
+    for a, b in zip(qk_norm_rope(k, k, w, w, cs, cs, at.to(dtype)), qk_norm_rope(k, k, w, w, cs, cs, at.int())):
+        assert torch.equal(a, b)
     assert _lib.debug_status() == 0

@@ -252,6 +252,17 @@ def launch(device: int, fn, *args) -> None:
         check(rc)
 
 
+INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def int32(t: torch.Tensor) -> torch.Tensor:
+    """``t``, a tensor of integers (no other type is cut to one), as int32, its strides as they come."""
+    if t.dtype == torch.int32:
+        return t
+    assert t.dtype in INTEGERS, f"{t.dtype} where integers are needed"
+    return t.to(torch.int32)
+
+
 def int64s(*values: int):
     """``values`` as a ctypes int64 array (strides kept with a checked set of shapes)."""
     return (ctypes.c_int64 * len(values))(*values)

@@ -64,7 +64,7 @@ def _rows(t: torch.Tensor):
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else _lib.int32(t).contiguous()
 
 
 def paged_kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,
@@ -138,7 +138,7 @@ def paged_attention_kv4(q: torch.Tensor, cache: torch.Tensor, block_tables: torc
     if t == 0 or hq == 0:
         return out
     q, sq = _rows(q)
-    bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
+    bt = _lib.int32(block_tables)
     cl, cu = _int32(context_lens), _int32(cu_seqlens)
     max_new = min(int(max_new), t)
     lib = _lib.load()

@@ -47,11 +47,11 @@ def paged_plan(block_tables: torch.Tensor, seq_lens: torch.Tensor, n_new: torch.
     assert free_blocks.get_device() == device and block_size >= 1 and max_tokens >= 0
     assert free_start is None or (free_start.numel() == 1 and free_start.get_device() == device)
     max_tokens = int(max_tokens)
-    sl, nn, fb = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    sl, nn, fb = (t if t.dtype == torch.int32 and t.is_contiguous() else _lib.int32(t).contiguous()
                   for t in (seq_lens, n_new, free_blocks))
     out = block_tables.new_empty((2 * max_tokens + 2 * b + 2,))
     at = out.data_ptr()
-    fs = None if free_start is None else free_start.to(torch.int32)
+    fs = None if free_start is None else _lib.int32(free_start)
     _lib.launch(device, _lib.load().tllm_paged_plan_from, block_tables.data_ptr(), sl.data_ptr(),
                 nn.data_ptr(), fb.data_ptr(), None if fs is None else fs.data_ptr(), at, at + 4 * max_tokens, at + 8 * max_tokens,
                 at + 4 * (2 * max_tokens + b + 1), at + 4 * (2 * max_tokens + 2 * b + 1), b,

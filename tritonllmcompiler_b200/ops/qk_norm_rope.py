@@ -63,7 +63,7 @@ def _checked(q, sq, k, sk, wq, swq, wk, swk, cos, scos, sin, ssin, pos, spos, dt
     assert len(cos) == 2 and cos[1] == d // 2 and sin == cos
     assert cos_dtype == torch.float32 and sin_dtype == torch.float32
     axes = 1 if len(pos) == 1 else pos[0]
-    assert len(pos) in (1, 2) and pos[-1] == t
+    assert len(pos) in (1, 2) and pos[-1] == t and pos_dtype in _lib.INTEGERS
     sections = (d // 2,) if sections is None else sections
     assert axes == len(sections), "one row of positions per section"
     words = _axis_words(sections, interleaved, d // 2)
@@ -105,7 +105,8 @@ def _readable(tensors):
     def fix(i, x):
         s = x.stride()
         if i == 6:
-            return x.to(torch.int32) if s[-1] == 1 else x.to(torch.int32).clone(memory_format=torch.contiguous_format)
+            x = _lib.int32(x)
+            return x if x.stride()[-1] == 1 else x.clone(memory_format=torch.contiguous_format)
         ok = s == (1,) if i in (2, 3) else _table_ok(s) if i in (4, 5) else _rows_ok(s)
         return x if ok and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
