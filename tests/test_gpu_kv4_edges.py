@@ -326,3 +326,33 @@ def test_integers_of_other_sizes(cuda_device, dtype):
     for a, b in zip(qk_norm_rope(k, k, w, w, cs, cs, at.to(dtype)), qk_norm_rope(k, k, w, w, cs, cs, at.int())):
         assert torch.equal(a, b)
     assert _lib.debug_status() == 0
+
+
+def test_integers_past_32_bits_do_not_wrap(cuda_device):
+    """Slots, blocks and positions of 2^32 and more are outside everything, not inside after wrapping; lengths are
+    as long as the table."""
+    case = _case(25, [20], [2], 1, 2, 64, 16, F)
+    q, cache, table, ctx, cu, k, v = (t.cuda() for t in case)
+    before = cache.clone()
+    bad = torch.tensor([2 ** 32, 2 ** 32 + 5, -2 ** 32, -2 ** 33 + 1, 2 ** 31], device="cuda")
+    paged_kv4_append(k[:5], v[:5], cache, bad, block_size=16)
+    torch.cuda.synchronize()
+    assert torch.equal(cache, before) and _lib.debug_status() == 0x200
+    gk, gv = paged_kv4_gather(cache, bad, block_size=16)
+    torch.cuda.synchronize()
+    assert (gk == 0).all() and (gv == 0).all() and _lib.debug_status() == 0x200
+    attend = lambda t, c: paged_attention_kv4(q, cache, t, c, cu, 2, block_size=16)  # noqa: E731
+    attend(table.long() + 2 ** 32, ctx)
+    torch.cuda.synchronize()
+    assert _lib.debug_status() == 0x200
+    full = torch.full_like(ctx, 32)
+    assert torch.equal(attend(table, ctx.long() + 2 ** 32).nan_to_num(7.0), attend(table, full).nan_to_num(7.0))
+    assert _lib.debug_status() == 0
+    plan = paged_plan(table.clone(), ctx.long() + 2 ** 32, ctx // ctx, table[0], block_size=16, max_tokens=1)
+    assert plan.slots.tolist() == [-1] and plan.new_lens.tolist() == [2 ** 31 - 1] and plan.taken.tolist() == [0]
+    w, cs = torch.ones(64, dtype=F, device="cuda"), torch.rand(32, 32, device="cuda")
+    at = torch.arange(20, device="cuda")
+    got = qk_norm_rope(k, k, w, w, cs, cs, at + 2 ** 32)
+    torch.cuda.synchronize()
+    assert _lib.debug_status() == 0x200
+    assert torch.equal(got[0], qk_norm_rope(k, k, w, w, cs, cs, at * 0)[0])

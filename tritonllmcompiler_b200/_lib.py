@@ -256,10 +256,13 @@ INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
 def int32(t: torch.Tensor) -> torch.Tensor:
-    """``t``, a tensor of integers (no other type is cut to one), as int32, its strides as they come."""
+    """``t``, a tensor of integers (no other type is cut to one), as int32, its strides as they come. A value
+    past int32 becomes the nearest one, which the kernels check as any other: it must not wrap to some index."""
     if t.dtype == torch.int32:
         return t
     assert t.dtype in INTEGERS, f"{t.dtype} where integers are needed"
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(torch.int32)
 
 
