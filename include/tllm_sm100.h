@@ -509,7 +509,8 @@ TLLM_API int tllm_qk_norm_rope_bwd(const void *dq_out, const void *dk_out, const
  * no room for, a NaN or an infinity: all of it reads back as NaN, and rows that see it get NaN in its channels.)
  *
  * tllm_paged_kv4_append quantises k and v [T, Hkv, D] (strides sk/sv {token, head}) into slots
- * [T] (block * block_size + offset; negative: skipped; past the pool: skipped and reported through
+ * [T] (block * block_size + offset; negative: skipped; past the pool, or 2^31 - 1, which
+ * tllm_paged_plan gives for slots that int32 has no number for: skipped and reported through
  * tllm_debug_status). tllm_paged_kv4_gather writes the values that slots hold into k and v (zeros
  * for slots that hold nothing).
  */

@@ -356,3 +356,21 @@ def test_integers_past_32_bits_do_not_wrap(cuda_device):
     torch.cuda.synchronize()
     assert _lib.debug_status() == 0x200
     assert torch.equal(got[0], qk_norm_rope(k, k, w, w, cs, cs, at * 0)[0])
+
+
+def test_slots_past_32_bits(cuda_device):
+    """Blocks whose slots int32 has no number for: the plan gives one slot for all of them, and nothing is
+    written there (here a pool of 2^31 slots over the memory of one block)."""
+    table = torch.full((1, 2), 2 ** 27 + 3, dtype=torch.int32, device="cuda")
+    n = lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")  # noqa: E731
+    plan = paged_plan(table, n(5), n(3), n(0), block_size=16, max_tokens=3)
+    assert plan.slots.tolist() == [2 ** 31 - 1] * 3
+    one = torch.zeros(1, 1, 1, 1280, dtype=torch.uint8, device="cuda")
+    cache = one.expand(2 ** 27, 1, 1, 1280)
+    k = torch.randn(3, 1, 64, dtype=F, device="cuda")
+    paged_kv4_append(k, k, cache, plan.slots, block_size=16)
+    torch.cuda.synchronize()
+    assert (one == 0).all() and _lib.debug_status() == 0x200
+    paged_kv4_append(k, k, cache, plan.slots - 1, block_size=16)
+    torch.cuda.synchronize()
+    assert not (one == 0).all() and _lib.debug_status() == 0

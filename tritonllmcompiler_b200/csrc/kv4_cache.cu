@@ -25,6 +25,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "kv4.cuh"
 #include "ptx.cuh"
@@ -292,7 +294,8 @@ int entry(const char *op, bool append, const void *k, const void *v, void *cache
   a.T = T;
   a.H = static_cast<int>(H);
   a.log2_bs = block_size == 16 ? 4 : (block_size == 32 ? 5 : 6);
-  a.num_slots = num_blocks * block_size;
+  // The largest slot stands for all those that int32 has no number for (paged_plan saturates).
+  a.num_slots = std::min<int64_t>(num_blocks * block_size, INT32_MAX);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == TLLM_DTYPE_F16) return D == 64 ? launch<__half, 64>(a, append, st) : launch<__half, 128>(a, append, st);
   return D == 64 ? launch<__nv_bfloat16, 64>(a, append, st) : launch<__nv_bfloat16, 128>(a, append, st);
