@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from tritonllmcompiler_b200 import _lib
 
@@ -167,6 +168,7 @@ class _QkNormRope(torch.autograd.Function):
         return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, **ctx.how)
 
     @staticmethod
+    @once_differentiable  # a second derivative is an error, not left out of a sum
     def backward(ctx, dq_out, dk_out):
         grads = qk_norm_rope_backward(dq_out, dk_out, *ctx.saved_tensors, **ctx.how)
         return (*grads, None, None, None, None, None, None)
@@ -174,6 +176,6 @@ class _QkNormRope(torch.autograd.Function):
 
 def qk_norm_rope_train(q, k, q_weight, k_weight, cos, sin, positions, *, sections=None,
                        interleaved=False, eps: float = 1e-6):
-    """``qk_norm_rope`` with a backward pass (torch autograd) for q, k and the two weights."""
+    """``qk_norm_rope`` with a backward pass (torch autograd, once) for q, k and the two weights."""
     return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved,
                              eps)
