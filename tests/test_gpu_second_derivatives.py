@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tritonllmcompiler_b200.ops.flash_backward import flash_attention_train
 from tritonllmcompiler_b200.ops.qk_norm_rope import qk_norm_rope_train
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +22,9 @@ def test_qk_norm_rope(cuda_device):
     at = torch.arange(4, dtype=torch.int32, device="cuda")
     for leaf in (q, k, w):
         _refused(qk_norm_rope_train(q, k, w, w, cos, sin, at), leaf)
+
+
+def test_flash_attention(cuda_device):
+    q, k, v = (torch.randn(1, 2, 128, 64, dtype=torch.float16, device="cuda", requires_grad=True) for _ in range(3))
+    for leaf in (q, k, v):
+        _refused([flash_attention_train(q, k, v, causal=True)], leaf)

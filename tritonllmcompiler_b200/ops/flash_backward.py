@@ -9,6 +9,7 @@ extensions: the package root and ``ops`` keep the reference's four exports.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from tritonllmcompiler_b200 import _lib
 
@@ -84,6 +85,7 @@ class _FlashAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable  # a second derivative is an error, not left out of a sum
     def backward(ctx, dout):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = flash_attention_backward(q, k, v, o, lse, dout, causal=ctx.causal,
@@ -92,5 +94,5 @@ class _FlashAttention(torch.autograd.Function):
 
 
 def flash_attention_train(q, k, v, *, causal: bool = False, sm_scale: float | None = None):
-    """``flash_attention`` with a backward pass (torch autograd)."""
+    """``flash_attention`` with a backward pass (torch autograd, once)."""
     return _FlashAttention.apply(q, k, v, causal, sm_scale)
