@@ -532,7 +532,7 @@ TLLM_API int tllm_paged_kv4_gather(const void *cache, const int32_t *slots, void
  * before cu_seqlens[0] or past cu_seqlens[B] give zeros. A sequence with more than max_new tokens is
  * reported through tllm_debug_status, and its tokens past the first max_new give NaN. Block-table entries outside the pool read block 0 and are
  * reported through tllm_debug_status. workspace: tllm_paged_kv4_attn_workspace_size bytes,
- * 256-byte aligned (0 when no launch splits the keys).
+ * 256-byte aligned (0 only where there is nothing to attend for: no rows, or shapes that the call refuses).
  */
 TLLM_API size_t tllm_paged_kv4_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
                                                    int64_t max_new, int64_t D, int64_t block_size,

@@ -3,7 +3,7 @@
 //
 // A block (page) of one KV head is block_size / 16 pieces of 16 tokens, 20 * D bytes each and
 // contiguous: one bulk copy brings everything attention needs of those tokens. Groups of 32
-// channels of one token share a scale and a zero (fp16): value = code * scale + zero.
+// channels of one token share a scale and a zero (fp16): value = code * scale + zero (a scale that is NaN: a group without numbers).
 //   [ 0 D,  8 D)  K codes, D / 2 bytes per token. The 32-bit word [lane 4][w D / 32] holds channels
 //                 32 w + 8 lane + j, channel j at bits 4 (j / 2) + 16 (j % 2): lane c of a quad
 //                 reads its codes of all groups in one vector, and a mask of two nibbles at

@@ -37,15 +37,18 @@ constexpr int kStages = 2;  // tiles of a warp in shared memory
 constexpr int kMergeLoads = 8;  // parts a merging warp reads at a time
 constexpr int kMinTiles = 2;  // a warp's least run of tiles
 // Places of the line that a segment's queries, results and start take (64 and 300 requests of 512 .. 8192 keys, four
-// of 100,000: none 109, 386 and 192 us, 3 103, 370 and 187, 4 103, 364 and 187, 6 103, 368 and 185).
+// of 65,536 .. 131,072 with up to 32 rows, from a cold L2: none 110, 390 and 194 us, 3 105, 368 and 191, 4 103, 365 and
+// 191, 6 103, 368 and 187).
 constexpr int kExtra = 4;
 // Query rows per sequence and KV head up to which kv4_split_kernel runs. 64 requests of 512 .. 8192 keys, split
-// and prefill kernel: 16 rows 159 and 259 us, 32 rows 294 and 261, 48 rows 421 and 263; four of 100,000 keys,
-// 32 rows: 271 and 290.
+// and prefill kernel: 16 rows 163 and 265 us, 32 rows 300 and 268, 48 rows 429 and 271; four of 100,000 keys,
+// 32 rows: 286 and 294. (Rows alone, so a batch of many requests with 17 to 32 rows each is up to 12 % from the
+// better of the two.)
 constexpr int kSplitRows = 32;
 
-// CTAs of the split kernel per SM: what its registers allow without spilling much (two row tiles of 8 in
-// 168 registers, three CTAs, took 175 us where 157 do; one in 128, four CTAs, 135 where 123 did).
+// CTAs of the split kernel per SM: what its registers allow without spilling much. One row tile of 8 (64 requests of
+// 512 .. 8192 keys, a row tile of 4 rows): three CTAs 103 us, four, in 128 registers, 112. Two (the same requests with
+// 16 rows; four of 65,536 .. 131,072 keys): two CTAs 163 and 189 us, three, in 168 registers, 179 and 212.
 __host__ __device__ constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
 
 // Units of the products with the codes (fp16 subnormals) and with the zeros. The sums of q are split into two fp16
@@ -109,7 +112,8 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 //           fp16 again after the scale (packed products on the transposed weights, a third of the
 //           instructions of fp32 ones). The second sum is one more MMA. The 8 centres both sums on
 //           0: without it two sums of twice the size cancel, with 2.4 times the rounding errors, and over
-//           100,000 keys the MMAs' truncating sums alone doubled the error of a bf16 output. For fp16
+//           100,000 keys the MMAs' truncating sums alone doubled the error of a bf16 output. (z + 8 s is rounded
+//           to fp16, an error of 2^-12 of the group's middle.) For fp16
 //           outputs the low parts that the rounding after the scale leaves out are multiplied too
 //           (error 1.4 times that of rounding the output, against 1.6, for 5 % of the time).
 // Weights are 2^(x - mu) with mu = m - k: k <= 12 keeps the weights times the scales in fp16's normal
@@ -117,9 +121,11 @@ __device__ __forceinline__ void spread(uint32_t w, uint32_t (&x)[4]) {
 // when it grows by more than 2^3 (weights and products stay under 2^15).
 // An S^T result becomes a P^T operand by transposing 8 x 8 blocks in registers (movmatrix).
 //
-// Bound: HBM by bytes (1.25 D per token and head), but what holds it now is turning codes into operands:
-// 64 decode steps of U[512, 8192] keys, 32 heads over 8 of 128, fp16: 101 us, 3.9 TB/s; four requests of
-// 65,536 .. 131,072 keys with up to 32 rows: 180 us, half of the issue slots and 39 % of the tensor pipe.
+// Bound: HBM by bytes (1.25 D per token and head), but nothing is saturated: latency between the few warps that the
+// registers allow holds it. 64 decode steps of U[512, 8192] keys, 32 heads over 8 of 128, fp16: 101 us, 3.9 TB/s, with
+// 11 warps an SM half of the HBM's peak, 55 % of the issue slots, 45 % of the integer and 33 % of the tensor pipe; four
+// requests of 65,536 .. 131,072 keys with up to 32 rows: 183 us, with 8 warps half of the issue slots and 38 % of the
+// tensor pipe (each code is turned into operands once for 16 rows).
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, resident(NT)) kv4_split_kernel(const Args a) {
   using P = Piece<D>;

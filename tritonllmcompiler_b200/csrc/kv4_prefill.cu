@@ -11,6 +11,9 @@
 //                 buffers (the next tile's overlaps this tile's softmax), O += P V with P from TMEM
 //   warps 0-7     two threads per query row, 64 keys of a tile each: q to fp16 (bf16 rows by a power of
 //                 two that keeps them in its range), softmax with a lazy rescale of O (2^8), results
+// K, V and the weights are fp16 operands, rounded once each (2^-12 of a value, 2^-12 of a weight). With fp16 outputs
+// that doubles the error of rounding the output alone, and scores are off by some 2^-12 of their spread: by 0.005 where
+// they have a standard deviation of 29 (K of size 8, q of size 4). bf16 outputs do not show it.
 // V's columns are stored in the order 0 4 1 5 2 6 3 7 of every eight channels (the order in which one
 // mask yields pairs) and put right where O is read. The V rows of a last tile past the context are
 // zeros. A V group whose scale, zero or largest value (15 s + z) is no fp16 number is stored as zeros too and
@@ -19,8 +22,8 @@
 //
 // Bound: tensor products, 4 Hq D flops per visible pair, if K and V were 16-bit. They are 4-bit, so each tile
 // of 128 keys is unpacked for every 128 rows: 8 requests of up to 512 new tokens in up to 4096, 32 heads over
-// 8 of 128, bf16: 183 us, 458 TFLOP/s. A tile takes 3200 cycles, 2800 of them each for its softmax and,
-// beside it, its unpacking; half of the issue slots, 42 % of the integer pipe and a quarter of the tensor
+// 8 of 128, bf16: 177 us, 472 TFLOP/s. A tile takes some 3200 cycles, 2800 of them each for its softmax and,
+// beside it, its unpacking; half of the issue slots, 43 % of the integer pipe and a quarter of the tensor
 // pipe are busy, so latency between few warps holds it. What was slower on the same requests: part of the powers
 // of two by a polynomial (+9 to 15 %), twice the unpacking warps (+15 %), a row's 64 scores in registers at
 // once (+6 %), two row tiles a CTA that share a tile's unpacking (+27 %).
@@ -52,7 +55,7 @@ namespace {
 constexpr int BM = kPrefillRows;
 constexpr int BN = 128;
 // Places of the line that a segment's queries, results and empty pipeline take: 13,000 cycles, tiles 3,200 each.
-// (8 requests of up to 512 new tokens in up to 4096: none 226 us, 2 199, 3 195, 4 187, 5 187.)
+// (8 requests of up to 512 new tokens in up to 4096, from a cold L2: none 224 us, 2 196, 3 190, 4 184, 5 183.)
 constexpr int kExtra = 4;
 constexpr int kPieces = BN / kPieceTokens;
 constexpr int kRowThreads = 256;  // two per query row

@@ -12,7 +12,8 @@
 // Work: 8 bytes out per token and 16 per sequence; at one decode step nothing but latency, so
 // everything is one launch: each CTA scans (n, need) over all B sequences itself (B values from
 // L2, a few hundred ns) instead of a second launch or a grid-wide wait, then finds its tokens'
-// sequences by bisection of the scan in shared memory. 64 decode steps take 4.2 us of the GPU.
+// sequences by bisection of the scan in shared memory. 64 decode steps take 3.2 us of the
+// GPU (calls in a graph), 509 sequences with 64 K new tokens 11.6.
 #include "common.h"
 
 namespace tllm {
